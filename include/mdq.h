@@ -46,7 +46,8 @@ typedef enum mdq_dtype {
     MDQ_I16 = 4,
     MDQ_U16 = 5,
     MDQ_I32 = 6,
-    MDQ_U32 = 7
+    MDQ_U32 = 7,
+    MDQ_I64 = 8      /* token and vocabulary indices (mdq_ops.h) */
 } mdq_dtype;
 
 /*

@@ -19,7 +19,7 @@ MDQ_ERR_CUDA = 3
 MDQ_ERR_TOO_LARGE = 4
 
 # mdq_dtype
-MDQ_F32, MDQ_BF16, MDQ_I8, MDQ_U8, MDQ_I16, MDQ_U16, MDQ_I32, MDQ_U32 = range(8)
+MDQ_F32, MDQ_BF16, MDQ_I8, MDQ_U8, MDQ_I16, MDQ_U16, MDQ_I32, MDQ_U32, MDQ_I64 = range(9)
 
 # mdq_layout
 LAYOUT_PACKED4, LAYOUT_S8U8, LAYOUT_S16U16, LAYOUT_S32U32, LAYOUT_M8V4 = range(5)
@@ -91,6 +91,63 @@ class StepOptions(ctypes.Structure):
                 ("grad_delta", ctypes.c_int64 * 8)]
 
 
+# mdq_norm_kind
+NORM_RMS, NORM_LAYER = 0, 1
+
+DISTILL_MAX_TOP = 1024
+
+
+class EmbedDesc(ctypes.Structure):
+    """Mirror of ``mdq_embed_desc``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "ids", "out")] + [
+        (n, ctypes.c_int64) for n in ("tokens", "vocab", "dim", "table_stride")] + [
+        ("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("table_dtype", "out_dtype", "ids_dtype")]
+
+
+class EmbedGradDesc(ctypes.Structure):
+    """Mirror of ``mdq_embed_grad_desc``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("grad_out", "ids", "grad", "workspace")] + [
+        (n, ctypes.c_int64) for n in ("workspace_bytes", "tokens", "vocab", "dim",
+                                      "grad_out_stride", "padding_idx")] + [
+        ("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("grad_out_dtype", "grad_dtype", "ids_dtype", "accumulate",
+                                      "reserved")]
+
+
+class ResidualNormDesc(ctypes.Structure):
+    """Mirror of ``mdq_residual_norm_desc``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "h", "x_new", "n", "stats", "post_weight",
+                                               "post_bias", "pre_weight", "pre_bias", "gate")] + [
+        (n, ctypes.c_int64) for n in ("rows", "dim", "x_stride", "h_stride", "gate_rows")] + [
+        (n, ctypes.c_float) for n in ("residual_scale", "eps")] + [
+        (n, ctypes.c_int32) for n in ("x_dtype", "h_dtype", "param_dtype", "kind")]
+
+
+class ResidualNormGradDesc(ctypes.Structure):
+    """Mirror of ``mdq_residual_norm_grad_desc``."""
+
+    _fields_ = [("f", ResidualNormDesc)] + [
+        (n, ctypes.c_void_p) for n in ("grad_new", "grad_n", "grad_x", "grad_h",
+                                       "grad_post_weight", "grad_post_bias", "grad_pre_weight",
+                                       "grad_pre_bias", "grad_gate", "workspace")] + [
+        (n, ctypes.c_int64) for n in ("workspace_bytes", "grad_new_stride", "grad_n_stride")]
+
+
+class TopkDistillDesc(ctypes.Structure):
+    """Mirror of ``mdq_topk_distill_desc``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "teacher", "index", "weight", "upstream",
+                                               "row_loss", "loss", "grad")] + [
+        (n, ctypes.c_int64) for n in ("rows", "vocab", "logits_stride", "grad_stride",
+                                      "upstream_stride")] + [
+        ("top", ctypes.c_int32), ("temperature", ctypes.c_float), ("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("logits_dtype", "teacher_dtype", "index_dtype")]
+
+
 class MDQError(RuntimeError):
     """A non-zero mdq_status, with the library's message."""
 
@@ -126,6 +183,18 @@ _SIGNATURES = {
                                                     ctypes.c_void_p]),
     "mdq_fakequant_adamw_multi": (ctypes.c_int, [ctypes.POINTER(FQDesc), ctypes.c_int32,
                                                  ctypes.c_void_p]),
+    # Operators (mdq_ops.h).  Descriptors travel as packed bytes (ops.py).
+    "mdq_embed": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "mdq_embed_grad_workspace_bytes": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64,
+                                                      ctypes.c_int64,
+                                                      ctypes.POINTER(ctypes.c_int64)]),
+    "mdq_embed_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "mdq_residual_norm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "mdq_residual_norm_grad_workspace_bytes": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64,
+                                                              ctypes.c_int64,
+                                                              ctypes.POINTER(ctypes.c_int64)]),
+    "mdq_residual_norm_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "mdq_topk_distill": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "mdq_last_error": (ctypes.c_char_p, []),
     "mdq_abi_version": (ctypes.c_int32, []),
 }

@@ -26,7 +26,7 @@ SOURCES = ["mdq_step.cu", "mdq_stats.cu", "mdq_tiles_packed4.cu", "mdq_tiles_s8u
            "mdq_tiles_s16u16.cu", "mdq_tiles_s32u32.cu", "mdq_tiles_m8v4.cu",
            "mdq_blocks_packed4.cu", "mdq_blocks_s8u8.cu", "mdq_blocks_s16u16.cu",
            "mdq_blocks_s32u32.cu", "mdq_blocks_m8v4.cu", "mdq_staged_s8u8.cu", "mdq_staged_packed4.cu",
-           "mdq_fakequant.cu"]
+           "mdq_fakequant.cu", "mdq_embed.cu", "mdq_norm.cu", "mdq_distill.cu"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -40,7 +40,7 @@ def nvcc() -> str:
 def _inputs() -> list[str]:
     files = [os.path.join(CSRC, s) for s in SOURCES]
     files += [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    files.append(os.path.join(INCLUDE, "mdq.h"))
+    files += [os.path.join(INCLUDE, h) for h in ("mdq.h", "mdq_ops.h")]
     return files
 
 
