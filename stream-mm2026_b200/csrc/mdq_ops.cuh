@@ -51,4 +51,92 @@ inline mdq_status launch_status(const char* what) {
                             : mdq_fail(MDQ_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 
+// 16 bytes of T as floats and back.
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    __device__ static __forceinline__ void unpack(uint4 w, float (&v)[4]) {
+        v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y);
+        v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+    }
+    __device__ static __forceinline__ uint4 pack(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                          __float_as_uint(v[3]));
+    }
+};
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&p);
+}
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    __device__ static __forceinline__ void unpack(uint4 w, float (&v)[8]) {
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    }
+    __device__ static __forceinline__ uint4 pack(const float (&v)[8]) {
+        return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                          pack_bf16(v[6], v[7]));
+    }
+};
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+inline int64_t type_size(int32_t t) { return t == MDQ_BF16 ? 2 : 4; }
+// Whether rows `stride` elements apart from `p` on all start on 16 bytes.
+inline bool rows16(const void* p, int64_t stride, int32_t type) {
+    return aligned16(p) && stride * type_size(type) % 16 == 0;
+}
+inline int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
+
+// One launch.  With `dependent` the grid may be set up while the previous
+// kernel of the stream still runs; it calls wait_previous() before it reads
+// what that kernel wrote (programmatic dependent launch).
+template <typename... P, typename... A>
+inline cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                          cudaStream_t stream, int cluster, bool dependent, A... args) {
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(
+            reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+            (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchAttribute at[2];
+    unsigned n = 0;
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = (unsigned)cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (dependent) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    c.attrs = at;
+    c.numAttrs = n;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
+
+// Until the previous kernel of the stream has ended and its writes are visible
+// (at once when this kernel was not launched as dependent).
+__device__ __forceinline__ void wait_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+inline mdq_status status_of(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return MDQ_OK;
+    cudaGetLastError();   // the error is reported here, not by a later launch
+    return mdq_fail(MDQ_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+}
+
 }  // namespace mdq_ops
