@@ -42,6 +42,12 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
 inline bool float_type(int32_t t) { return t == MDQ_F32 || t == MDQ_BF16; }
 inline bool id_type(int32_t t) { return t == MDQ_I32 || t == MDQ_I64; }
 
@@ -92,16 +98,20 @@ inline bool rows16(const void* p, int64_t stride, int32_t type) {
 }
 inline int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
 
+// Dynamic shared memory a kernel may ask for (227 KB less its static arrays,
+// which stay below 1 KB).
+constexpr int kMaxShared = 226 * 1024;
+
 // One launch.  With `dependent` the grid may be set up while the previous
 // kernel of the stream still runs; it calls wait_previous() before it reads
 // what that kernel wrote (programmatic dependent launch).
 template <typename... P, typename... A>
 inline cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
                           cudaStream_t stream, int cluster, bool dependent, A... args) {
-    if (smem > 48 * 1024) {
+    if (smem > 48 * 1024) {   // always the same limit: calls of other threads may set it as well
         const cudaError_t e = cudaFuncSetAttribute(
             reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-            (int)smem);
+            kMaxShared);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchAttribute at[2];
