@@ -36,54 +36,210 @@ __device__ __forceinline__ Stat merge(Stat a, Stat b) {
     return {h, a.s * ex2(a.h - k) + b.s * ex2(b.h - k)};
 }
 
-// The teacher's entries of a row, in the block's shared memory.
+// The teacher's entries of a row, in shared memory.
 struct Teacher {
     int* idx;       // [top] vocabulary index, -1 absent
     float* q;       // [top] probability
     float* lq;      // [top] its logarithm
     float* sum;     // [top] probabilities of all entries with this index; -1 if an earlier has it
-    float* z;       // [top] the student's logits there (rank 0 only)
-};
-
-// ---------------------------------------------------------------- whole rows
-
-// A row stays in the shared memory of a cluster of CTAs while its maximum, its
-// sum and its gradient are formed, so the logits are read from memory once and
-// the gradient is written once: the pass is bound by that traffic (two
-// exponentials an element take about 0.7 of its time with bf16 logits).  Each
-// CTA holds a slice of whole 16-byte units, brought by bulk copies in kStages
-// parts so that the sum starts with the first; the CTAs' maxima and sums meet
-// through distributed shared memory.  More CTAs a row where it does not fit in
-// half an SM's shared memory, or where few rows would leave SMs idle.
-constexpr int kStages = 4, kMaxCluster = 8;
-
-struct RowShared {
-    unsigned long long bar[kStages];
-    Stat warp[kWarps];
-    Stat cta[kMaxCluster];
-    int live;
-};
-
-__device__ __forceinline__ unsigned smem_at(const void* p) {
-    return (unsigned)__cvta_generic_to_shared(p);
-}
-
-// A copy of a few KB lands in microseconds; the limit (hundreds of
-// milliseconds) only keeps a lost one from hanging the GPU.
-__device__ __forceinline__ bool wait_copy(unsigned bar) {
-    for (int i = 0; i < 1 << 22; ++i) {
-        unsigned done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], 0;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(bar) : "memory");
-        if (done) return true;
+    float* z;       // [top] the student's logits there
+    __device__ Teacher(char* p, int top) {
+        idx = reinterpret_cast<int*>(p);
+        q = reinterpret_cast<float*>(idx) + top;
+        lq = q + top;
+        sum = lq + top;
+        z = sum + top;
     }
-    return false;
+};
+constexpr int kTeacherBytes = 20;   // of an entry
+
+// Bits in which entries of a row mark their index, to find repeated ones.
+constexpr int kMarkWords = 512;
+
+// The entries of row r, by one warp: the teacher's distribution, the student's
+// logits at the entries (with `gather`), and for each index its first entry
+// with the sum of the probabilities of all that share it (with `sums`).
+// Returns whether the teacher has an entry.
+template <typename T>
+__device__ __forceinline__ bool teacher_row(const mdq_topk_distill_desc& d, int64_t r, const T* z,
+                                            const Teacher& K, bool gather, bool sums,
+                                            unsigned* marks, int lane) {
+    const float it = 1.0f / d.temperature;
+    const bool i64 = d.index_dtype == MDQ_I64, bf16 = d.teacher_dtype == MDQ_BF16;
+    const auto entry = [&](int k, int& i, float& t) {
+        const int64_t v = load_id(d.index, i64, r * d.top + k);
+        t = load_any(d.teacher, bf16, r * d.top + k);
+        const bool in = v >= 0 && v < d.vocab;
+        if (!in) t = -CUDART_INF_F;
+        i = in ? (int)v : -1;
+    };
+    // A NaN is an entry: the row becomes NaN.
+    const auto larger = [](float m, float t) { return fmaxf(m, t != t ? 0.0f : t); };
+    if (d.top <= 32) {   // an entry a lane
+        int i = -1;
+        float t = -CUDART_INF_F, zi = 0.0f;
+        if (lane < d.top) entry(lane, i, t);
+        if (gather && i >= 0) zi = to_f(z[i]);
+        const float tm = warp_max(larger(-CUDART_INF_F, t));
+        if (tm == -CUDART_INF_F) return false;
+        const float l = (t - tm) * it, e = i < 0 ? 0.0f : expf(l), s = warp_sum(e);
+        const float q = e * (1.0f / s);
+        float sum = q;
+        const unsigned same = __match_any_sync(0xffffffffu, i);
+        for (unsigned others = same & (same - 1); __any_sync(0xffffffffu, others != 0);
+             others &= others - 1) {   // those behind the first, in order
+            const float more = __shfl_sync(0xffffffffu, q, others != 0 ? __ffs(others) - 1 : lane);
+            if (others != 0) sum += more;
+        }
+        if (lane < d.top) {
+            K.idx[lane] = i;
+            K.q[lane] = q;
+            K.lq[lane] = l - logf(s);
+            K.sum[lane] = i >= 0 && (same & ((1u << lane) - 1)) == 0 ? sum : -1.0f;
+            K.z[lane] = zi;
+        }
+        return true;
+    }
+    float tm = -CUDART_INF_F;
+    for (int k = lane; k < d.top; k += 32) {
+        int i;
+        float t;
+        entry(k, i, t);
+        K.idx[k] = i;
+        K.lq[k] = t;
+        tm = larger(tm, t);
+    }
+    tm = warp_max(tm);
+    if (tm == -CUDART_INF_F) return false;
+    float s = 0.0f;
+    for (int k = lane; k < d.top; k += 32) {
+        const float l = (K.lq[k] - tm) * it;
+        K.lq[k] = l;
+        s += K.q[k] = K.idx[k] < 0 ? 0.0f : expf(l);
+    }
+    s = warp_sum(s);
+    const float ls = logf(s), is = 1.0f / s;
+    for (int k = lane; k < d.top; k += 32) {
+        K.q[k] *= is;
+        K.lq[k] -= ls;
+    }
+    if (gather) {
+#pragma unroll 4
+        for (int k = lane; k < d.top; k += 32) K.z[k] = K.idx[k] < 0 ? 0.0f : to_f(z[K.idx[k]]);
+    }
+    if (sums) {
+        // Entries that find their index's bit set share it with another, or only
+        // the bit: for those the whole list is looked through.
+        for (int k = lane; k < kMarkWords; k += 32) marks[k] = 0;
+        __syncwarp();
+        for (int k0 = 0; k0 < d.top; k0 += 32) {
+            const int k = k0 + lane, i = k < d.top ? K.idx[k] : -1;
+            bool maybe = false;
+            if (i >= 0) {
+                const unsigned h = (unsigned)i * 2654435761u >> 18;   // 14 bits
+                maybe = atomicOr(&marks[h >> 5], 1u << (h & 31)) >> (h & 31) & 1;
+            }
+            if (k < d.top) K.sum[k] = i >= 0 ? K.q[k] : -1.0f;
+            __syncwarp();
+            for (unsigned m = __ballot_sync(0xffffffffu, maybe); m != 0; m &= m - 1) {
+                const int same = __shfl_sync(0xffffffffu, i, __ffs(m) - 1);
+                float sum = 0.0f;
+                int first = d.top;
+                for (int j = lane; j < min(d.top, k0 + 32); j += 32)
+                    if (K.idx[j] == same) {
+                        first = min(first, j);
+                        sum += K.q[j];
+                    }
+                sum = warp_sum(sum);
+                first = __reduce_min_sync(0xffffffffu, first);
+                for (int j = lane; j < min(d.top, k0 + 32); j += 32)
+                    if (K.idx[j] == same) K.sum[j] = j == first ? sum : -1.0f;
+                __syncwarp();
+            }
+        }
+    }
+    return true;
 }
 
-// 16 bytes of a slice that start `shift` bytes (4 words + half) behind unit u.
+// 2^(v c - shift) of a unit's elements, two products an instruction.
+template <int N>
+__device__ __forceinline__ void exponentials(float (&v)[N], float c, float shift) {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        asm("{\n\t.reg .b64 a, b, d;\n\t"
+            "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 d, {%3, %3};\n\t"
+            "fma.rn.f32x2 a, a, b, d;\n\tmov.b64 {%0, %1}, a;\n\t}"
+            : "+f"(v[j]), "+f"(v[j + 1]) : "f"(c), "f"(-shift));
+        v[j] = ex2(v[j]);
+        v[j + 1] = ex2(v[j + 1]);
+    }
+}
+template <int N>
+__device__ __forceinline__ float largest(const float (&v)[N]) {
+    float m[N / 4];
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j)
+        m[j] = fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3]));
+#pragma unroll
+    for (int j = 1; j < N / 4; ++j) m[0] = fmaxf(m[0], m[j]);
+    return m[0];
+}
+template <int N>
+__device__ __forceinline__ float total(const float (&v)[N]) {
+    float s[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int j = 4; j < N; ++j) s[j & 3] += v[j];
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+template <int N>
+__device__ __forceinline__ void add_values(Stat& a, float (&v)[N], float c) {
+    const float h = fmaxf(a.h, __fmul_rn(largest(v), c)), shift = finite_max(h);
+    exponentials(v, c, shift);
+    a = {h, fmaf(a.s, ex2(a.h - shift), total(v))};
+}
+
+// Adds units first, first + threads, ... below end, four at a time.
+template <typename T>
+__device__ __forceinline__ void add_units(Stat& a, const uint4* units, int first, int end,
+                                          int threads, float c) {
+    constexpr int N = Vec<T>::N;
+    int u = first;
+    for (; u + 3 * threads < end; u += 4 * threads) {
+        float v[4 * N];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            Vec<T>::unpack(units[u + j * threads], *reinterpret_cast<float(*)[N]>(v + j * N));
+        add_values(a, v, c);
+    }
+    for (; u + threads < end; u += 2 * threads) {
+        float v[2 * N];
+        Vec<T>::unpack(units[u], *reinterpret_cast<float(*)[N]>(v));
+        Vec<T>::unpack(units[u + threads], *reinterpret_cast<float(*)[N]>(v + N));
+        add_values(a, v, c);
+    }
+    if (u < end) {
+        float v[N];
+        Vec<T>::unpack(units[u], v);
+        add_values(a, v, c);
+    }
+}
+
+__device__ __forceinline__ Stat merge_warp(Stat a) {
+    float h = a.h;
+    asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(h));
+    return {h, warp_sum(a.s * ex2(a.h - finite_max(h)))};
+}
+
+// The loss of a row, by one warp.
+__device__ __forceinline__ float row_loss(const Teacher& K, int top, Stat a, float c, int lane) {
+    const float le = logf(a.s), shift = finite_max(a.h);
+    float l = 0.0f;
+    for (int k = lane; k < top; k += 32)
+        if (K.q[k] != 0.0f) l += K.q[k] * (K.lq[k] - (fmaf(K.z[k], c, -shift) * kLn2 - le));
+    return warp_sum(l);
+}
+
+// 16 bytes of shared memory from word `at` on, or from half a word behind it.
 __device__ __forceinline__ uint4 shifted(const uint32_t* words, int at, bool half) {
     uint32_t w[5];
 #pragma unroll
@@ -93,221 +249,229 @@ __device__ __forceinline__ uint4 shifted(const uint32_t* words, int at, bool hal
                       __funnelshift_r(w[2], w[3], 16), __funnelshift_r(w[3], w[4], 16));
 }
 
+// The softmax's part of the gradient, pe exp2(z c - shift), of `count` elements
+// that lie in `part` from element at0 on: elements up to a 16-byte boundary of
+// the gradient, whole units, the rest.  Where the boundaries of the gradient
+// are not those of the logits, a unit is put together from two.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) distill_rows(const __grid_constant__
-                                                            mdq_topk_distill_desc d,
-                                                            int slice_units) {
+__device__ __forceinline__ void write_part(T* to, const char* part, int at0, int count, float pe,
+                                           float c, float shift, int tid, int threads) {
+    constexpr int N = Vec<T>::N;
+    const int head = min(count, (int)((-(uintptr_t)to & 15) / sizeof(T)));
+    const int body = (count - head) / N, tail = count - head - body * N;
+    const int from = at0 + head;   // place of the first whole unit
+    const T* src = reinterpret_cast<const T*>(part) + at0;
+    const auto edge = [&](int i) { to[i] = from_f<T>(pe * ex2(fmaf(to_f(src[i]), c, -shift))); };
+    if (tid < head) edge(tid);
+    if (tid >= 16 && tid < 16 + tail) edge(head + body * N + tid - 16);
+    uint4* to16 = reinterpret_cast<uint4*>(to + head);
+    const auto unit = [&](uint4 x) {
+        float v[N];
+        Vec<T>::unpack(x, v);
+        exponentials(v, c, shift);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] *= pe;
+        return Vec<T>::pack(v);
+    };
+    if (from % N == 0) {
+        const uint4* units = reinterpret_cast<const uint4*>(part) + from / N;
+#pragma unroll 2
+        for (int u = tid; u < body; u += threads) __stcs(to16 + u, unit(units[u]));
+    } else {
+        const int byte = from * (int)sizeof(T);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(part) + byte / 4;
+        const bool half = byte % 4 != 0;
+        for (int u = tid; u < body; u += threads) __stcs(to16 + u, unit(shifted(words, 4 * u, half)));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_zeros(T* to, int64_t count, int tid, int threads) {
+    const int head = (int)min(count, (int64_t)((-(uintptr_t)to & 15) / sizeof(T)));
+    const int64_t body = (count - head) / Vec<T>::N;
+    const int tail = (int)(count - head - body * Vec<T>::N);
+    if (tid < head) to[tid] = from_f<T>(0.0f);
+    if (tid >= 16 && tid < 16 + tail) to[head + body * Vec<T>::N + tid - 16] = from_f<T>(0.0f);
+    for (int64_t u = tid; u < body; u += threads)
+        __stcs(reinterpret_cast<uint4*>(to + head) + u, make_uint4(0, 0, 0, 0));
+}
+
+// ------------------------------------------------------------------- copying
+
+__device__ __forceinline__ unsigned smem_at(const void* p) {
+    return (unsigned)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void bar_init(void* bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_at(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(void* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory");
+}
+
+// Whether the barrier's phase ended.  Phases last microseconds; the limit
+// (hundreds of milliseconds) only keeps a lost copy from hanging the GPU.
+__device__ __forceinline__ bool bar_wait(void* bar, unsigned parity) {
+    for (int i = 0; i < 1 << 22; ++i) {
+        unsigned done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(smem_at(bar)), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ unsigned long long read_once() {   // evict-first in L2
+    unsigned long long policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+// Arrives at the barrier with a copy of `bytes` (may be 0) that ends on it.
+__device__ __forceinline__ void copy_in(void* bar, void* to, const void* from, unsigned bytes,
+                                        unsigned long long policy) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes)
+                 : "memory");
+    if (bytes > 0)
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1], %2, [%3], %4;" ::"r"(smem_at(to)),
+            "l"(from), "r"(bytes), "r"(smem_at(bar)), "l"(policy)
+            : "memory");
+}
+
+// The 16-byte units a row of logits lies in, counted from the boundary at or
+// before its start; `lead` elements of the first precede the row.
+template <typename T>
+struct RowUnits {
+    static constexpr int N = Vec<T>::N;
+    const T* z;
+    int64_t vocab, units;
+    int lead;
+    __device__ RowUnits(const mdq_topk_distill_desc& d, int64_t r)
+        : z(static_cast<const T*>(d.logits) + r * d.logits_stride), vocab(d.vocab) {
+        lead = (int)(((uintptr_t)z & 15) / sizeof(T));
+        units = (lead + vocab + N - 1) / N;
+    }
+    // First element of unit u (negative for the first), and those of a part.
+    __device__ int64_t element(int64_t u) const { return u * N - lead; }
+    __device__ int64_t begin(int64_t u0) const { return max((int64_t)0, element(u0)); }
+    __device__ int64_t end(int64_t u1) const { return min(vocab, element(u1)); }
+    // Whether the unit holds elements that are not the row's: those are not
+    // copied in bulk but element by element.
+    __device__ bool shared(int64_t u) const {
+        return (u == 0 && lead > 0) || element(u + 1) > vocab;
+    }
+    // The value in place t of unit u, -infinity outside of the row.
+    __device__ T value(int64_t u, int t) const {
+        const int64_t e = element(u) + t;
+        return e >= 0 && e < vocab ? z[e] : from_f<T>(-CUDART_INF_F);
+    }
+};
+
+// ------------------------------------------------------------------ few rows
+
+// A row stays in the shared memory of a cluster of CTAs, a slice each, so that
+// few rows use many SMs.  Bulk copies bring a slice in kParts parts and the sum
+// starts with the first; the CTAs' statistics meet through distributed shared
+// memory.
+constexpr int kParts = 4, kMaxCluster = 8;
+
+struct RowShared {
+    unsigned long long bar[kParts];
+    Stat warp[kWarps];
+    Stat cta[kMaxCluster];
+    unsigned marks[kMarkWords];
+    int live;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) distill_cluster(const __grid_constant__
+                                                               mdq_topk_distill_desc d,
+                                                               int slice_units) {
     extern __shared__ __align__(16) char raw[];
     __shared__ RowShared S;
     constexpr int N = Vec<T>::N;   // elements of a unit
     T* slice = reinterpret_cast<T*>(raw);
-    Teacher K;
-    K.idx = reinterpret_cast<int*>(raw + 16 * (size_t)(slice_units + 1));
-    K.q = reinterpret_cast<float*>(K.idx) + d.top;
-    K.lq = K.q + d.top;
-    K.sum = K.lq + d.top;
-    K.z = K.sum + d.top;
+    const Teacher K(raw + 16 * (size_t)(slice_units + 1), d.top);
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
     const int64_t r = blockIdx.x / C;
-    const T* z = static_cast<const T*>(d.logits) + r * d.logits_stride;
+    const RowUnits<T> row(d, r);
     T* out = d.grad == nullptr ? nullptr : static_cast<T*>(d.grad) + r * d.grad_stride;
-
-    // Units of the row count from the 16-byte boundary at or before its start;
-    // `lead` elements of the first precede the row.  This CTA's slice: units
-    // [u0, u1), elements [e0, e1) of the row.
-    const int lead = (int)(((uintptr_t)z & 15) / sizeof(T));
-    const int64_t units = (lead + d.vocab + N - 1) / N;
-    const int64_t u0 = min(units, (int64_t)rank * slice_units);
-    const int64_t u1 = min(units, u0 + slice_units);
-    const int64_t e0 = max((int64_t)0, u0 * N - lead), e1 = min(d.vocab, u1 * N - lead);
+    // This CTA's slice: units [u0, u1).
+    const int64_t u0 = min(row.units, (int64_t)rank * slice_units);
+    const int64_t u1 = min(row.units, u0 + slice_units);
     const int n = (int)(u1 - u0);
 
     const float w = d.weight == nullptr ? 1.0f : d.weight[r];
     bool live = w != 0.0f;
     if (tid == 0) {
 #pragma unroll
-        for (int k = 0; k < kStages; ++k)
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_at(&S.bar[k])) : "memory");
+        for (int k = 0; k < kParts; ++k) bar_init(&S.bar[k], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // The others of the cluster run before their shared memory is written to.
     auto started = cluster.barrier_arrive();
-    const int per = (n + kStages - 1) / kStages;   // units of a stage
+    const int per = (n + kParts - 1) / kParts;   // units of a part
+    const bool first_shared = n > 0 && row.shared(u0), last_shared = n > 0 && row.shared(u1 - 1);
     if (tid == 0 && live) {
-        // Whole units inside the row by bulk copies; a unit that the row shares
-        // with what lies before or behind it by elements, below.
-        const int first = u0 == 0 && lead > 0 ? 1 : 0;
-        const int last = u1 * N - lead > d.vocab ? n - 1 : n;
-        unsigned long long policy;
-        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+        const unsigned long long policy = read_once();
 #pragma unroll
-        for (int k = 0; k < kStages; ++k) {
-            const int a = max(first, k * per), b = min(last, (k + 1) * per);
-            const unsigned bytes = b > a ? (unsigned)(b - a) * 16u : 0u, bar = smem_at(&S.bar[k]);
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                         : "memory");
-            if (bytes > 0)
-                asm volatile(
-                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-                    " [%0], [%1], %2, [%3], %4;" ::"r"(smem_at(raw) + 16u * (unsigned)a),
-                    "l"(z + (u0 + a) * N - lead), "r"(bytes), "r"(bar), "l"(policy)
-                    : "memory");
+        for (int k = 0; k < kParts; ++k) {
+            const int a = max(first_shared ? 1 : 0, k * per), b = min(last_shared ? n - 1 : n, (k + 1) * per);
+            copy_in(&S.bar[k], raw + 16 * (size_t)a, row.z + row.element(u0 + a),
+                    b > a ? (unsigned)(b - a) * 16u : 0u, policy);
         }
     }
-    // The shared units' elements; -infinity outside of the row.
-    if (live && n > 0) {
-        if (tid < N && u0 == 0 && lead > 0)
-            slice[tid] = tid >= lead && tid - lead < d.vocab ? z[tid - lead] : from_f<T>(-CUDART_INF_F);
-        if (tid >= 32 && tid < 32 + N && u1 * N - lead > d.vocab && !(u0 == 0 && lead > 0 && n == 1)) {
-            const int64_t e = (u1 - 1) * N - lead + tid - 32;
-            slice[(n - 1) * N + tid - 32] = e < d.vocab ? z[e] : from_f<T>(-CUDART_INF_F);
-        }
-    }
-    // The teacher's distribution, by the last warp.
-    const float it = 1.0f / d.temperature, c = it * kLog2e;
-    if (live && warp == (threads >> 5) - 1) {
-        float tm = -CUDART_INF_F;
-        for (int k = lane; k < d.top; k += 32) {
-            const int64_t i = load_id(d.index, d.index_dtype == MDQ_I64, r * d.top + k);
-            float t = load_any(d.teacher, d.teacher_dtype == MDQ_BF16, r * d.top + k);
-            const bool in = i >= 0 && i < d.vocab;
-            if (!in) t = -CUDART_INF_F;
-            K.idx[k] = in ? (int)i : -1;
-            K.lq[k] = t;
-            if (rank == 0) K.z[k] = in ? to_f(z[i]) : 0.0f;
-            tm = fmaxf(tm, t != t ? 0.0f : t);   // a NaN is an entry: the row becomes NaN
-        }
-        tm = warp_max(tm);
-        float s = 0.0f;
-        for (int k = lane; k < d.top; k += 32) {
-            const float l = (K.lq[k] - tm) * it;
-            K.lq[k] = l;
-            s += K.q[k] = K.idx[k] < 0 ? 0.0f : expf(l);
-        }
-        s = warp_sum(s);
-        const float ls = logf(s), is = 1.0f / s;
-        for (int k = lane; k < d.top; k += 32) {
-            K.q[k] *= is;
-            K.lq[k] -= ls;
-        }
-        if (lane == 0) S.live = tm != -CUDART_INF_F;
+    if (live && first_shared && tid < N) slice[tid] = row.value(u0, tid);
+    if (live && last_shared && tid >= 32 && tid < 32 + N)
+        slice[(n - 1) * N + tid - 32] = row.value(u1 - 1, tid - 32);
+    const float c = 1.0f / d.temperature * kLog2e;
+    if (live && warp == (threads >> 5) - 1) {   // the teacher, by the last warp
+        const bool has = teacher_row(d, r, row.z, K, rank == 0, out != nullptr, S.marks, lane);
+        if (lane == 0) S.live = has;
     }
     __syncthreads();
     live = live && S.live != 0;
-    // Entries that share an index: the first carries their sum.
-    if (live && out != nullptr)
-        for (int k = tid; k < d.top; k += threads) {
-            const int i = K.idx[k];
-            float sum = 0.0f;
-            bool first = i >= 0;
-            for (int j = 0; j < d.top; ++j)
-                if (K.idx[j] == i) {
-                    first = first && j >= k;
-                    sum += K.q[j];
-                }
-            K.sum[k] = first ? sum : -1.0f;
-        }
 
-    // Maximum and sum of this thread's units, two at a time.
     Stat a = {-CUDART_INF_F, 0.0f};
-    const uint4* units16 = reinterpret_cast<const uint4*>(raw);
+    const uint4* units = reinterpret_cast<const uint4*>(raw);
     bool arrived = true;
     if (w != 0.0f)   // also where the teacher has nothing: the copies end in this CTA's time
-        for (int k = 0; k < kStages; ++k) {
-            arrived &= wait_copy(smem_at(&S.bar[k]));
-            if (!live) continue;
-            const int end = min(n, (k + 1) * per);
-            for (int u = k * per + tid; u < end; u += 2 * threads) {
-                float v[2 * N];
-                Vec<T>::unpack(units16[u], *reinterpret_cast<float(*)[N]>(v));
-                if (u + threads < end) {
-                    Vec<T>::unpack(units16[u + threads], *reinterpret_cast<float(*)[N]>(v + N));
-                } else {
-#pragma unroll
-                    for (int j = N; j < 2 * N; ++j) v[j] = -CUDART_INF_F;
-                }
-                float m = v[0];
-#pragma unroll
-                for (int j = 1; j < 2 * N; ++j) m = fmaxf(m, v[j]);
-                const float h = fmaxf(a.h, __fmul_rn(m, c)), shift = finite_max(h);
-                float s = a.s * ex2(a.h - shift);
-#pragma unroll
-                for (int j = 0; j < 2 * N; ++j) s += ex2(fmaf(v[j], c, -shift));
-                a = {h, s};
-            }
+        for (int k = 0; k < kParts; ++k) {
+            arrived &= bar_wait(&S.bar[k], 0);
+            if (live) add_units<T>(a, units, k * per + tid, min(n, (k + 1) * per), threads, c);
         }
     if (!arrived) a.s = CUDART_NAN_F;   // the row's results become NaN
     // All threads, all CTAs.
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        a = merge(a, {__shfl_xor_sync(0xffffffffu, a.h, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+    a = merge_warp(a);
     if (lane == 0) S.warp[warp] = a;
     cluster.barrier_wait(std::move(started));
     __syncthreads();
     if (warp == 0) {
-        a = lane < threads >> 5 ? S.warp[lane] : Stat{-CUDART_INF_F, 0.0f};
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            a = merge(a, {__shfl_xor_sync(0xffffffffu, a.h, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+        a = merge_warp(lane < threads >> 5 ? S.warp[lane] : Stat{-CUDART_INF_F, 0.0f});
         if (lane < C) *cluster.map_shared_rank(&S.cta[rank], lane) = a;
     }
     if (C > 1) cluster.sync();
     else __syncthreads();
     a = S.cta[0];
     for (int k = 1; k < C; ++k) a = merge(a, S.cta[k]);
-    const float shift = finite_max(a.h), scale = d.scale * w;
 
+    const float scale = d.scale * w;
     if (rank == 0 && warp == 0 && d.row_loss != nullptr) {
-        const float le = logf(a.s);
-        float l = 0.0f;
-        if (live)
-            for (int k = lane; k < d.top; k += 32)
-                if (K.q[k] != 0.0f) l += K.q[k] * (K.lq[k] - (fmaf(K.z[k], c, -shift) * kLn2 - le));
-        l = warp_sum(l);
-        if (lane == 0)
-            d.row_loss[r] = live ? d.temperature * d.temperature * scale * l : 0.0f;
+        const float l = live ? d.temperature * d.temperature * scale * row_loss(K, d.top, a, c, lane)
+                             : 0.0f;
+        if (lane == 0) d.row_loss[r] = l;
     }
-    if (out == nullptr) return;
-
+    const int64_t e0 = row.begin(u0), e1 = row.end(u1);
+    if (out == nullptr || e1 <= e0) return;
+    if (!live) return write_zeros(out + e0, e1 - e0, tid, threads);
     const float up = d.upstream == nullptr ? 1.0f : d.upstream[r * d.upstream_stride];
-    const float f = live ? up * scale * d.temperature : 0.0f, pe = live ? f / a.s : 0.0f;
-    // Elements up to a 16-byte boundary of the gradient, whole units, the rest.
-    const int64_t count = e1 - e0;
-    if (count <= 0) return;
-    T* to = out + e0;
-    const int at0 = (int)(e0 - (u0 * N - lead));   // place of e0 in the slice
-    const int head = (int)min(count, (int64_t)((-(uintptr_t)to & 15) / sizeof(T)));
-    const int body = (int)((count - head) / N), tail = (int)(count - head) - body * N;
-    const int from = at0 + head;                   // place of the first whole unit
-    const auto edge = [&](int i) {
-        to[i] = from_f<T>(live ? pe * ex2(fmaf(to_f(slice[at0 + i]), c, -shift)) : 0.0f);
-    };
-    if (tid < head) edge(tid);
-    if (tid >= 32 && tid < 32 + tail) edge(head + body * N + tid - 32);
-    uint4* to16 = reinterpret_cast<uint4*>(to + head);
-    if (!live) {
-        for (int u = tid; u < body; u += threads) __stcs(to16 + u, make_uint4(0, 0, 0, 0));
-        return;
-    }
-    const auto unit = [&](uint4 x) {
-        float v[N];
-        Vec<T>::unpack(x, v);
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = pe * ex2(fmaf(v[j], c, -shift));
-        return Vec<T>::pack(v);
-    };
-    if (from % N == 0) {   // the gradient's units are the logits'
-        const uint4* src = units16 + from / N;
-#pragma unroll 2
-        for (int u = tid; u < body; u += threads) __stcs(to16 + u, unit(src[u]));
-    } else {
-        const int byte = from * (int)sizeof(T);
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(raw) + byte / 4;
-        const bool half = byte % 4 != 0;
-        for (int u = tid; u < body; u += threads) __stcs(to16 + u, unit(shifted(words, 4 * u, half)));
-    }
+    const float f = up * scale * d.temperature, pe = f / a.s, shift = finite_max(a.h);
+    const int at0 = (int)(e0 - row.element(u0));   // place of e0 in the slice
+    write_part(out + e0, raw, at0, (int)(e1 - e0), pe, c, shift, tid, threads);
     __syncthreads();
     // The teacher's entries of this slice, over what was stored there.
     for (int k = tid; k < d.top; k += threads) {
@@ -318,106 +482,362 @@ __global__ void __launch_bounds__(kThreads, 2) distill_rows(const __grid_constan
     }
 }
 
-// ----------------------------------------------------------------- long rows
+// ----------------------------------------------------------------- many rows
 
-// Rows that no cluster can hold: three passes over memory, one block a row.
-__device__ __forceinline__ float block_max(float v) {
-    __shared__ float red[kWarps];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) v = fmaxf(v, red[i]);
-    return v;
+// Persistent CTAs.  Rows go to them in turn; where rows have weights, those of
+// weight 0 (which cost a third of the others') go round separately, so that
+// every CTA gets its share of both.  The whole 16-byte units of a row are divided among the warps; every warp brings its slice of the next rows
+// in pieces through a ring of its own in shared memory and refills a piece as
+// soon as it is done with it, so that copies run ahead without the warps
+// waiting for one another.  They meet once a row, when their maxima and sums
+// are joined.  The last `stages` pieces of a slice stay in the ring until the
+// gradient has been formed from them; pieces of a slice that is longer are
+// brought a second time, from L2 as a rule.  With the loss alone, pieces are
+// refilled at once.  One more warp looks up the teacher's entries some rows
+// ahead and forms the rows' losses behind.
+struct StreamPlan {
+    int warps;         // that share a row
+    int each;          // 16-byte units of a warp's slice
+    int piece_units;   // 16-byte units of a piece
+    int stages;        // pieces of a warp's ring
+    int depth;         // rows whose entries are kept
+    int listed;        // places of a CTA's list of rows; 0: every gridDim-th row
+};
+constexpr int kMaxStages = 8, kMaxDepth = 4;
+
+// Waits that ran out.
+__device__ unsigned int g_distill_timeouts;
+
+// A place in a ring: its stage, and the phase its barriers are in.
+struct Place {
+    int stage = 0;
+    unsigned phase = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+struct StreamShared {
+    unsigned long long full[kWarps][kMaxStages];
+    unsigned long long told[kMaxDepth], heard[kMaxDepth];   // entries are there, are done with
+    int live[kMaxDepth];
+    Stat stat[kMaxDepth];
+    Stat warp[2][kWarps];
+    unsigned marks[kMarkWords];
+    int part[kWarps + 1];
+};
+
+__device__ __forceinline__ float row_weight(const mdq_topk_distill_desc& d, int64_t r) {
+    return d.weight == nullptr ? 1.0f : __ldg(d.weight + r);
 }
-__device__ __forceinline__ float block_sum(float v) {
-    __shared__ float red[kWarps];
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
+
+// The rows of this CTA: `live` of weight other than 0, then `dead` of weight 0.
+struct Rows {
+    const int* list;   // nullptr: every gridDim-th
+    int64_t live, dead;
+    __device__ __forceinline__ int64_t at(int64_t i) const {
+        return list == nullptr ? blockIdx.x + i * gridDim.x : list[i];
+    }
+};
+
+// Fills the list: row r is the k-th of its kind, by the kinds of the rows before
+// it, and belongs to CTA k mod gridDim.  Every CTA counts for itself: the
+// weights come from L2.
+__device__ __forceinline__ Rows find_rows(const mdq_topk_distill_desc& d, int places, int* list,
+                                          int* part) {
+    if (places == 0) {
+        const int64_t b = blockIdx.x;
+        return {nullptr, (d.rows - b + gridDim.x - 1) / gridDim.x, 0};
+    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int rows = (int)d.rows, each = (rows + blockDim.x - 1) / blockDim.x;
+    const int r0 = min(rows, tid * each), r1 = min(rows, r0 + each);
+    int mine = 0;
+#pragma unroll 4
+    for (int r = r0; r < r1; ++r) mine += __ldg(d.weight + r) != 0.0f;
+    int upto = mine;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) v += red[i];
-    return v;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) part[warp] = upto;
+    __syncthreads();
+    int before = upto - mine, all = 0;
+    for (int k = 0; k < warps; ++k) {
+        if (k < warp) before += part[k];
+        all += part[k];
+    }
+    const int G = gridDim.x, b = blockIdx.x;
+    const int live = all > b ? (all - b + G - 1) / G : 0;
+    const int dead = rows - all > b ? (rows - all - b + G - 1) / G : 0;
+    int k = before, z = r0 - before;   // places of this thread's next rows, live and dead
+    int km = k % G, zm = z % G;
+    for (int r = r0; r < r1; ++r) {
+        if (__ldg(d.weight + r) != 0.0f) {
+            if (km == b) list[k / G] = r;
+            ++k;
+            if (++km == G) km = 0;
+        } else {
+            if (zm == b) list[live + z / G] = r;
+            ++z;
+            if (++zm == G) zm = 0;
+        }
+    }
+    __syncthreads();
+    return {list, live, dead};
+}
+
+// A row as the warps share it: `head` elements up to the first 16-byte
+// boundary, whole units, `tail` elements; warp w has `mine` units from `from` on.
+template <typename T>
+struct Share {
+    static constexpr unsigned N = Vec<T>::N;
+    const T* z;
+    int head, tail, mine, from;
+    __device__ __forceinline__ Share(const mdq_topk_distill_desc& d, const T* row, int first, int each)
+        : z(row) {   // first: the warp's first unit
+        const unsigned vocab = (unsigned)d.vocab;
+        head = (int)min(vocab, (unsigned)(-(uintptr_t)z & 15) / (unsigned)sizeof(T));
+        const unsigned rest = vocab - head, units = rest / N;
+        tail = (int)(rest % N);
+        mine = max(0, min((int)units - first, each));
+        from = head + first * (int)N;
+    }
+};
+
+// The entries' warp.
+template <typename T>
+__device__ __forceinline__ void stream_entries(const mdq_topk_distill_desc& d, const StreamPlan& P,
+                                               StreamShared& S, const Rows& R, char* info,
+                                               int lane) {
+    const float c = 1.0f / d.temperature * kLog2e;
+    Place slots;
+    // The loss of the row whose entries are in the slot, once the others are done.
+    const auto finish = [&](int slot, int64_t r, unsigned phase) {
+        if (!bar_wait(&S.heard[slot], phase)) {
+            if (lane == 0) atomicAdd(&g_distill_timeouts, 1u);
+            return false;
+        }
+        if (d.row_loss == nullptr) return true;
+        const Teacher K(info + (size_t)slot * kTeacherBytes * d.top, d.top);
+        float l = 0.0f;
+        if (S.live[slot])
+            l = d.temperature * d.temperature * d.scale * row_weight(d, r) *
+                row_loss(K, d.top, S.stat[slot], c, lane);
+        if (lane == 0) d.row_loss[r] = l;
+        __syncwarp();
+        return true;
+    };
+    for (int64_t i = 0; i < R.live; ++i) {
+        const int64_t r = R.at(i);
+        const int slot = slots.stage;
+        if (i >= P.depth && !finish(slot, R.at(i - P.depth), slots.phase ^ 1)) return;
+        const Teacher K(info + (size_t)slot * kTeacherBytes * d.top, d.top);
+        const T* z = static_cast<const T*>(d.logits) + r * d.logits_stride;
+        const bool live = row_weight(d, r) != 0.0f &&
+                          teacher_row(d, r, z, K, true, d.grad != nullptr, S.marks, lane);
+        if (lane == 0) S.live[slot] = live;
+        __syncwarp();
+        if (lane == 0) bar_arrive(&S.told[slot]);
+        slots.next(P.depth);
+    }
+    if (d.row_loss == nullptr) return;
+    for (int64_t i = lane; i < R.dead; i += 32) d.row_loss[R.at(R.live + i)] = 0.0f;
+    if (R.live < P.depth) slots = {0, 1};
+    for (int64_t i = max((int64_t)0, R.live - P.depth); i < R.live; ++i, slots.next(P.depth))
+        if (!finish(slots.stage, R.at(i), slots.phase ^ 1)) return;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_long_rows(const __grid_constant__
-                                                         mdq_topk_distill_desc d) {
-    __shared__ int64_t idx[MDQ_DISTILL_MAX_TOP];
-    __shared__ float q[MDQ_DISTILL_MAX_TOP], lq[MDQ_DISTILL_MAX_TOP];
-    const int64_t r = blockIdx.x;
-    const T* z = static_cast<const T*>(d.logits) + r * d.logits_stride;
-    T* out = d.grad == nullptr ? nullptr : static_cast<T*>(d.grad) + r * d.grad_stride;
-    const float it = 1.0f / d.temperature, c = it * kLog2e;
-    const float w = d.weight == nullptr ? 1.0f : d.weight[r];
-    const float scale = d.scale * w;
-    float tm = -CUDART_INF_F;
-    if (w != 0.0f) {
-        for (int k = threadIdx.x; k < d.top; k += kThreads) {
-            int64_t i = load_id(d.index, d.index_dtype == MDQ_I64, r * d.top + k);
-            float t = load_any(d.teacher, d.teacher_dtype == MDQ_BF16, r * d.top + k);
-            if (i < 0 || i >= d.vocab) { i = -1; t = -CUDART_INF_F; }
-            idx[k] = i;
-            lq[k] = t;
-            tm = fmaxf(tm, t != t ? 0.0f : t);   // a NaN is an entry: the row becomes NaN
+__global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_constant__
+                                                                   mdq_topk_distill_desc d,
+                                                                   const __grid_constant__ StreamPlan P) {
+    extern __shared__ __align__(16) char raw[];
+    __shared__ StreamShared S;
+    constexpr int N = Vec<T>::N;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = P.warps;
+    const size_t piece_bytes = 16 * (size_t)P.piece_units, ring_bytes = piece_bytes * P.stages;
+    char* ring = raw + warp * ring_bytes;
+    char* info = raw + W * ring_bytes + 16;
+    if (tid == 0) {
+        for (int k = 0; k < W; ++k)
+            for (int j = 0; j < P.stages; ++j) bar_init(&S.full[k][j], 1);
+        for (int k = 0; k < P.depth; ++k) {
+            bar_init(&S.told[k], 1);
+            bar_init(&S.heard[k], W);
         }
-        tm = block_max(tm);
-    }
-    if (tm == -CUDART_INF_F) {   // weight 0, or a teacher without an entry
-        if (out != nullptr)
-            for (int64_t v = threadIdx.x; v < d.vocab; v += kThreads) out[v] = from_f<T>(0.0f);
-        if (threadIdx.x == 0 && d.row_loss != nullptr) d.row_loss[r] = 0.0f;
-        return;
-    }
-    float s = 0.0f;
-    for (int k = threadIdx.x; k < d.top; k += kThreads) {
-        lq[k] = (lq[k] - tm) * it;
-        q[k] = expf(lq[k]);
-        s += q[k];
-    }
-    s = block_sum(s);
-    const float ls = logf(s), is = 1.0f / s;
-    for (int k = threadIdx.x; k < d.top; k += kThreads) {
-        q[k] *= is;
-        lq[k] -= ls;
-    }
-    float m = -CUDART_INF_F, e = 0.0f;
-    for (int64_t v = threadIdx.x; v < d.vocab; v += kThreads) m = fmaxf(m, to_f(z[v]));
-    m = block_max(m);
-    const float shift = m * c;
-    for (int64_t v = threadIdx.x; v < d.vocab; v += kThreads) e += exp2f(fmaf(to_f(z[v]), c, -shift));
-    e = block_sum(e);
-    const float le = logf(e);
-    float l = 0.0f;
-    for (int k = threadIdx.x; k < d.top; k += kThreads)
-        if (q[k] != 0.0f) l += q[k] * (lq[k] - ((to_f(z[idx[k]]) - m) * it - le));
-    l = block_sum(l);
-    if (threadIdx.x == 0 && d.row_loss != nullptr)
-        d.row_loss[r] = d.temperature * d.temperature * scale * l;
-    if (out == nullptr) return;
-    const float u = d.upstream == nullptr ? 1.0f : d.upstream[r * d.upstream_stride];
-    const float f = u * scale * d.temperature, pe = f / e;
-    float own[(MDQ_DISTILL_MAX_TOP + kThreads - 1) / kThreads];
-    int slot = 0;
-    for (int k = threadIdx.x; k < d.top; k += kThreads, ++slot) {
-        // The gradient at the entry's index, its repetitions counted; read before any is written.
-        if (idx[k] < 0) continue;
-        float sum = 0.0f;
-        for (int j = 0; j < d.top; ++j) sum += idx[j] == idx[k] ? q[j] : 0.0f;
-        own[slot] = pe * exp2f(fmaf(to_f(z[idx[k]]), c, -shift)) - f * sum;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    for (int64_t v = threadIdx.x; v < d.vocab; v += kThreads)
-        out[v] = from_f<T>(pe * exp2f(fmaf(to_f(z[v]), c, -shift)));
-    __syncthreads();
-    slot = 0;
-    for (int k = threadIdx.x; k < d.top; k += kThreads, ++slot)
-        if (idx[k] >= 0) out[idx[k]] = from_f<T>(own[slot]);
+    const Rows R = find_rows(d, P.listed,
+                             reinterpret_cast<int*>(info + (size_t)P.depth * kTeacherBytes * d.top),
+                             S.part);
+    if (warp == W) return stream_entries<T>(d, P, S, R, info, lane);
+
+    const float c = 1.0f / d.temperature * kLog2e;
+    const bool want = d.grad != nullptr;
+    // Pieces of this warp's slice: a row has one of two numbers of units, by
+    // where it starts.
+    const int first = warp * P.each, full_units = (int)(d.vocab / N);
+    const auto mine_of = [&](int units) { return max(0, min(units - first, P.each)); };
+    const int most = mine_of(full_units);
+    const int most_pieces = (most + P.piece_units - 1) / P.piece_units;
+    const int less_pieces = (mine_of(full_units - 1) + P.piece_units - 1) / P.piece_units;
+    const auto pieces_of = [&](int units) { return units == most ? most_pieces : less_pieces; };
+    const T* logits = static_cast<const T*>(d.logits);
+    const unsigned long long policy = read_once();
+
+    // Copies: piece ik of `loads` of the row before the inext-th, to the place `to`.
+    const T* iz = nullptr;
+    int64_t inext = 0;
+    int ik = 0, loads = 0, in = 0, iunits = 0;
+    Place to;
+    const auto copy_next = [&] {
+        while (ik == loads) {
+            if (inext == R.live) return;
+            const Share<T> s(d, logits + R.at(inext) * d.logits_stride, first, P.each);
+            iz = s.z + s.from;
+            iunits = s.mine;
+            in = pieces_of(s.mine);
+            loads = in + (want && in > P.stages ? in - P.stages : 0);
+            ik = 0;
+            ++inext;
+        }
+        const int piece = ik < in ? ik : ik - in;
+        const int u = piece * P.piece_units, n = min(P.piece_units, iunits - u);
+        // The warp has read the piece that was here: the values went into results
+        // before the __syncwarp() ahead of this call.
+        if (lane == 0)
+            copy_in(&S.full[warp][to.stage], ring + to.stage * piece_bytes, iz + (int64_t)u * N,
+                    16u * (unsigned)n, policy);
+        ++ik;
+        to.next(P.stages);
+    };
+    for (int k = 0; k < P.stages; ++k) copy_next();
+
+    Place at, slots;
+    int parity = 0;
+    if (want)   // while the first copies are on their way
+        for (int64_t i = 0; i < R.dead; ++i)
+            write_zeros(static_cast<T*>(d.grad) + R.at(R.live + i) * d.grad_stride, d.vocab, tid, 32 * W);
+    for (int64_t i = 0; i < R.live; ++i) {
+        const int64_t r = R.at(i);
+        const float w = row_weight(d, r);   // used behind the sum
+        T* out = want ? static_cast<T*>(d.grad) + r * d.grad_stride : nullptr;
+        const Share<T> s(d, logits + r * d.logits_stride, first, P.each);
+        // The elements outside of whole units, by the first warp.
+        const bool edge = warp == 0 && (lane < s.head || (lane >= 16 && lane < 16 + s.tail));
+        const int64_t edge_at = lane < s.head ? lane : d.vocab - s.tail + lane - 16;
+        float edge_value = -CUDART_INF_F;
+        if (edge) edge_value = to_f(s.z[edge_at]);
+
+        // ---- maximum and sum
+        const int n = pieces_of(s.mine), keep = want ? min(n, P.stages) : 0;
+        const Place begin = at;
+        Stat a = {-CUDART_INF_F, 0.0f};
+        bool arrived = true;
+        for (int k = 0; k < n; ++k, at.next(P.stages)) {
+            arrived &= bar_wait(&S.full[warp][at.stage], at.phase);
+            add_units<T>(a, reinterpret_cast<const uint4*>(ring + at.stage * piece_bytes), lane,
+                         min(P.piece_units, s.mine - k * P.piece_units), 32, c);
+            if (k < n - keep) {
+                __syncwarp();
+                copy_next();
+            }
+        }
+        if (edge) {
+            const float h = __fmul_rn(edge_value, c);
+            a = merge(a, {h, ex2(fmaf(edge_value, c, -finite_max(h)))});
+        }
+        const int slot = slots.stage;
+        arrived &= bar_wait(&S.told[slot], slots.phase);
+        if (!arrived) {   // the row's results become NaN
+            a.s = CUDART_NAN_F;
+            if (lane == 0) atomicAdd(&g_distill_timeouts, 1u);
+        }
+        a = merge_warp(a);
+        if (lane == 0) S.warp[parity][warp] = a;
+        asm volatile("bar.sync 1, %0;" ::"r"(32 * W) : "memory");
+        a = merge_warp(lane < W ? S.warp[parity][lane] : Stat{-CUDART_INF_F, 0.0f});
+        if (tid == 0) S.stat[slot] = a;
+        parity ^= 1;
+
+        if (want) {
+            // ---- gradient: the pieces in the ring, then those brought again
+            const bool live = S.live[slot] != 0;
+            const float up = d.upstream == nullptr ? 1.0f : __ldg(d.upstream + r * d.upstream_stride);
+            const float f = up * d.scale * w * d.temperature, pe = __fdividef(f, a.s);
+            const float shift = finite_max(a.h);
+            // The teacher's entries of this slice (the first of them, or all).
+            const Teacher K(info + (size_t)slot * kTeacherBytes * d.top, d.top);
+            const int end = s.from + s.mine * N;
+            const auto entry = [&](int k, int& i, float& v) {
+                i = -1;
+                if (k >= d.top) return;
+                const int at_index = K.idx[k];
+                const float sum = K.sum[k];
+                const bool own = (at_index >= s.from && at_index < end) ||
+                                 (warp == 0 && (at_index < s.head || at_index >= (int)d.vocab - s.tail));
+                if (sum < 0.0f || !own || !live) return;
+                i = at_index;
+                v = pe * ex2(fmaf(K.z[k], c, -shift)) - f * sum;
+            };
+            int entry_at = -1;
+            float entry_value = 0.0f;
+            entry(lane, entry_at, entry_value);
+            T* mine = out + s.from;
+            const bool same = ((uintptr_t)mine & 15) == 0;   // units of both are the same
+            // The first piece kept is where the slice began, or, when the slice
+            // took more than the ring, where the next piece is.
+            Place kept = n <= P.stages ? begin : at;
+            for (int k = 0; k < n; ++k) {
+                const int piece = k < keep ? n - keep + k : k - keep;
+                const int stage = k < keep ? kept.stage : at.stage;
+                if (k < keep) {
+                    kept.next(P.stages);
+                } else {
+                    bar_wait(&S.full[warp][stage], at.phase);
+                    at.next(P.stages);
+                }
+                const int u0 = piece * P.piece_units, count = min(P.piece_units, s.mine - u0);
+                const char* part = ring + stage * piece_bytes;
+                T* dst = mine + (int64_t)u0 * N;
+                if (!live) {
+                    write_zeros(dst, (int64_t)count * N, lane, 32);
+                } else if (same) {
+                    const uint4* units = reinterpret_cast<const uint4*>(part);
+#pragma unroll 2
+                    for (int u = lane; u < count; u += 32) {
+                        float v[N];
+                        Vec<T>::unpack(units[u], v);
+                        exponentials(v, c, shift);
+#pragma unroll
+                        for (int j = 0; j < N; ++j) v[j] *= pe;
+                        __stcs(reinterpret_cast<uint4*>(dst) + u, Vec<T>::pack(v));
+                    }
+                } else {
+                    write_part(dst, part, 0, count * N, pe, c, shift, lane, 32);
+                }
+                __syncwarp();
+                copy_next();
+            }
+            if (edge) out[edge_at] = from_f<T>(live ? pe * ex2(fmaf(edge_value, c, -shift)) : 0.0f);
+            __syncwarp();
+            // The entries, over what was stored there.
+            if (entry_at >= 0) out[entry_at] = from_f<T>(entry_value);
+            for (int k = lane + 32; k < d.top; k += 32) {
+                entry(k, entry_at, entry_value);
+                if (entry_at >= 0) out[entry_at] = from_f<T>(entry_value);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&S.heard[slot]);
+        slots.next(P.depth);
+    }
 }
 
 // The sum of the rows' losses, in a fixed order.
@@ -437,25 +857,46 @@ __global__ void __launch_bounds__(kThreads) distill_total(const float* rows, int
 
 template <typename T>
 mdq_status run_rows(const mdq_topk_distill_desc& d, cudaStream_t stream) {
-    // Bytes of shared memory beside the slice, and what a CTA may have: two CTAs
-    // an SM, or one for the longest rows.
-    const int64_t extra = 16 + 20 * (int64_t)d.top, half = 110 * 1024, whole = 222 * 1024;
     const int64_t units = ceil_div(d.vocab + Vec<T>::N - 1, Vec<T>::N);
+    const int64_t teacher = (int64_t)kTeacherBytes * d.top;
+    // At most one row an SM: clusters, with more CTAs a row while that fills
+    // idle SMs with 8 KB or more each.
     int cluster = 1;
-    const auto bytes = [&] { return 16 * ceil_div(units, cluster); };
-    while (cluster < kMaxCluster && bytes() + extra > half) cluster *= 2;
-    if (bytes() + extra > whole) {
-        distill_long_rows<T><<<(unsigned)d.rows, kThreads, 0, stream>>>(d);
-        return launch_status("distill");
+    const auto slice = [&] { return 16 * ceil_div(units, cluster); };
+    while (cluster < kMaxCluster && (slice() + 16 + teacher > 110 * 1024 ||
+                                     (d.rows * cluster <= 74 && slice() >= 16 * 1024)))
+        cluster *= 2;
+    if (d.rows <= 148 && slice() + 16 + teacher <= 222 * 1024) {
+        const int threads = slice() >= 16 * 1024 ? 512 : slice() >= 4 * 1024 ? 256 : 128;
+        return status_of(launch(distill_cluster<T>, dim3((unsigned)(d.rows * cluster)), threads,
+                                (size_t)(slice() + 16 + teacher), stream, cluster, false, d,
+                                (int)(slice() / 16)),
+                         "distill");
     }
-    // Few rows: more CTAs a row while that fills idle SMs with 8 KB or more each.
-    while (cluster < kMaxCluster && d.rows * cluster <= 74 && bytes() >= 16 * 1024) cluster *= 2;
-    const int64_t grid = d.rows * cluster;
-    if (grid > INT32_MAX) return mdq_fail(MDQ_ERR_TOO_LARGE, "distill: too many rows");
-    const int threads = bytes() >= 16 * 1024 ? 512 : bytes() >= 4 * 1024 ? 256 : 128;
-    return status_of(launch(distill_rows<T>, dim3((unsigned)grid), threads,
-                            (size_t)(bytes() + extra), stream, cluster, false, d,
-                            (int)(bytes() / 16)),
+    // Many rows.  8 warps a row and two CTAs an SM, so that one computes while
+    // the other joins its warps; 16 and one CTA where a row fills more than half
+    // of the shared memory; fewer warps for rows below 32 KB (4 KB a warp), and
+    // as many CTAs as the registers take.
+    // 16x1024 rows of 50257 bf16: 601 us with 8 warps, 718 with 16.
+    StreamPlan P;
+    P.warps = 1;
+    while (P.warps < 8 && 16 * units >= (int64_t)P.warps * 2 * 4096) P.warps *= 2;
+    if (d.grad != nullptr && 16 * units > 104 * 1024) P.warps = 16;
+    const int ctas = P.warps == 1 ? 10 : P.warps == 2 ? 7 : 16 / P.warps;
+    P.depth = teacher * kMaxDepth <= 8 * 1024 / ctas ? kMaxDepth : 2;
+    const int64_t grid = d.rows < 148 * ctas ? d.rows : 148 * ctas;
+    // Up to 65536 rows with weights are listed (two kinds, each rounded up).
+    P.listed = d.weight != nullptr && d.rows <= 65536 ? (int)(ceil_div(d.rows, grid) + 1) : 0;
+    // A ring of two pieces, each a whole slice where that fits.
+    P.each = (int)ceil_div(ceil_div(d.vocab, Vec<T>::N), P.warps);
+    P.stages = 2;
+    const int64_t beside = P.depth * teacher + 4 * (int64_t)P.listed + 16;
+    int64_t room = (218 * 1024 / ctas - 4608 - beside) / P.warps / 16 / P.stages;
+    if (room < 128) room = 128;   // long lists of entries beside short rows
+    P.piece_units = P.each < room ? P.each : (int)room;
+    const size_t smem = (size_t)(16 * P.piece_units * P.stages * P.warps + beside);
+    return status_of(launch(distill_stream<T>, dim3((unsigned)grid), 32 * P.warps + 32, smem, stream,
+                            1, false, d, P),
                      "distill");
 }
 

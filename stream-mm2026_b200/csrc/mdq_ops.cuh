@@ -99,8 +99,8 @@ inline bool rows16(const void* p, int64_t stride, int32_t type) {
 inline int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
 
 // Dynamic shared memory a kernel may ask for (227 KB less its static arrays,
-// which stay below 1 KB).
-constexpr int kMaxShared = 226 * 1024;
+// which stay below 4 KB).
+constexpr int kMaxShared = 223 * 1024;
 
 // One launch.  With `dependent` the grid may be set up while the previous
 // kernel of the stream still runs; it calls wait_previous() before it reads
