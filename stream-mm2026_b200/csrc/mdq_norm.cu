@@ -1,10 +1,10 @@
-// mdq_norm.cu - the norm after a block with its gate and the residual's scale,
-// and the norm before the next block (mdq_ops.h).
-#include "mdq_ops.cuh"
+// mdq_norm.cu - residual norm (mdq_ops.h): its entry points, the sums over CTAs,
+// and the kernels for rows that no cluster holds (the others: mdq_norm.cuh).
+#include "mdq_norm.cuh"
 
 namespace {
 
-using namespace mdq_ops;
+using namespace mdq_norm;
 
 constexpr int kThreads = 256;
 
@@ -46,7 +46,9 @@ struct Row {
     }
 };
 
-__global__ void __launch_bounds__(kThreads) norm_forward(const __grid_constant__
+// ------------------------------------------------- rows wider than a cluster
+
+__global__ void __launch_bounds__(kThreads) norm_wide(const __grid_constant__
                                                          mdq_residual_norm_desc d) {
     const Row R(d, blockIdx.x);
     const float inv = 1.0f / (float)d.dim;
@@ -118,7 +120,7 @@ struct Grad {
     }
 };
 
-__global__ void __launch_bounds__(kThreads) norm_backward_rows(const __grid_constant__
+__global__ void __launch_bounds__(kThreads) norm_grad_wide(const __grid_constant__
                                                                mdq_residual_norm_grad_desc g,
                                                                float* means) {
     const Grad G(g, blockIdx.x);
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_rows(const __grid_cons
 }
 
 // Gradients of one parameter column; `gate_row` >= 0: of that row of the gate.
-__global__ void __launch_bounds__(kThreads) norm_backward_columns(const __grid_constant__
+__global__ void __launch_bounds__(kThreads) norm_grad_wide_columns(const __grid_constant__
                                                                   mdq_residual_norm_grad_desc g,
                                                                   const float* means) {
     const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -188,6 +190,132 @@ __global__ void __launch_bounds__(kThreads) norm_backward_columns(const __grid_c
     if (g.grad_post_bias != nullptr) store_any(g.grad_post_bias, pb, c, b1);
     if (g.grad_pre_weight != nullptr) store_any(g.grad_pre_weight, pb, c, w2);
     if (g.grad_pre_bias != nullptr) store_any(g.grad_pre_bias, pb, c, b2);
+}
+
+// ------------------------------------------------------------- sums over CTAs
+
+// Adds the CTAs' sums of 32 columns, a warp every 16th CTA, and the warps' sums
+// in order; forms the parameters' gradients from them.  blockIdx.y: pre or post
+// norm.
+__global__ void __launch_bounds__(512) norm_grad_sum(const __grid_constant__
+                                                     mdq_residual_norm_grad_desc g,
+                                                     const __grid_constant__ Partials W, int blocks,
+                                                     int full, int grouped) {
+    __shared__ float red[2][16][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t dim = g.f.dim, c = (int64_t)blockIdx.x * 32 + lane;
+    const int kind = blockIdx.y;   // kPre or kPost; its bias is two further
+    wait_previous();
+    float s = 0.0f, b = 0.0f;
+    if (c < dim) {
+#pragma unroll 4
+        for (int i = warp; i < blocks; i += 16) {
+            s += W.sums[((int64_t)i * 4 + kind) * dim + c];
+            if (full) b += W.sums[((int64_t)i * 4 + kind + 2) * dim + c];
+        }
+    }
+    red[0][warp][lane] = s;
+    red[1][warp][lane] = b;
+    __syncthreads();
+    if (warp != 0 || c >= dim) return;
+    s = b = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        s += red[0][k][lane];
+        b += red[1][k][lane];
+    }
+    const bool pb = g.f.param_dtype == MDQ_BF16;
+    if (kind == kPre) {
+        if (g.grad_pre_weight != nullptr) store_any(g.grad_pre_weight, pb, c, s);
+        if (g.grad_pre_bias != nullptr) store_any(g.grad_pre_bias, pb, c, b);
+        return;
+    }
+    // One gate for all rows is applied here, and its gradient follows from the
+    // same sums; otherwise the rows applied theirs.
+    float gate = 1.0f;
+    if (!grouped && g.f.gate != nullptr) {
+        gate = load_any(g.f.gate, pb, c);
+        const float w = load_any(g.f.post_weight, pb, c);
+        const float bias = g.f.post_bias == nullptr ? 0.0f : load_any(g.f.post_bias, pb, c);
+        if (g.grad_gate != nullptr) store_any(g.grad_gate, pb, c, fmaf(w, s, bias * b));
+    }
+    if (g.grad_post_weight != nullptr) store_any(g.grad_post_weight, pb, c, gate * s);
+    if (g.grad_post_bias != nullptr) store_any(g.grad_post_bias, pb, c, gate * b);
+}
+
+// Rows of the gate whose group no team had whole: the teams' sums in order.
+__global__ void __launch_bounds__(256) norm_grad_gate(const __grid_constant__
+                                                      mdq_residual_norm_grad_desc g,
+                                                      const __grid_constant__ Partials W, int run,
+                                                      int full) {
+    const int64_t dim = g.f.dim, per = g.f.rows / g.f.gate_rows;
+    const bool pb = g.f.param_dtype == MDQ_BF16;
+    wait_previous();
+    for (int64_t k = blockIdx.y; k < g.f.gate_rows; k += gridDim.y) {
+        const int64_t first = k * per / run, last = ((k + 1) * per - 1) / run;   // teams
+        if (first == last) continue;
+        for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < dim; c += (int64_t)gridDim.x * 256) {
+            float s = 0.0f, b = 0.0f;
+#pragma unroll 4
+            for (int64_t i = first; i <= last; ++i) {
+                // The group began in the first of these teams and before the others.
+                const float* edge = W.edges + ((i * 2 + (i == first)) * 2) * dim;
+                s += edge[c];
+                if (full) b += edge[dim + c];
+            }
+            const float w = load_any(g.f.post_weight, pb, c);
+            const float bias = g.f.post_bias == nullptr ? 0.0f : load_any(g.f.post_bias, pb, c);
+            store_any(g.grad_gate, pb, k * dim + c, fmaf(w, s, bias * b));
+        }
+    }
+}
+
+// ------------------------------------------------------------------ planning
+
+// Columns a CTA takes, its threads, and the CTAs of a row; false when the row is
+// too wide for a cluster.
+bool plan_columns(int64_t dim, int* cluster, Teams* G) {
+    *cluster = 1;
+    while (*cluster < kMaxCluster && dim > (int64_t)*cluster * kTeam * kCols) *cluster *= 2;
+    if (dim > (int64_t)*cluster * kTeam * kCols) return false;
+    G->share = (int)(ceil_div(ceil_div(dim, *cluster), kCols) * kCols);
+    G->threads = (int)ceil_div(G->share, kCols * 32) * 32;
+    return true;
+}
+
+// The backward pass's teams, their rows, and what the workspace holds.
+struct GradPlan {
+    Teams G;
+    int cluster;
+    int64_t blocks;    // clusters, each with a row of sums
+    int64_t bytes;
+};
+bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, GradPlan* p) {
+    if (!plan_columns(dim, &p->cluster, &p->G)) return false;
+    Teams& G = p->G;
+    G.teams = p->cluster > 1 ? 1 : kTeam / G.threads;
+    // One CTA an SM (its registers end there), fewer where few rows would give
+    // teams less than four, so that the sums over CTAs stay short.
+    const int64_t most = 148 / p->cluster;
+    int64_t teams = ceil_div(rows, 4);
+    p->blocks = ceil_div(teams, G.teams);
+    if (p->blocks > most) p->blocks = most;
+    if (p->blocks < 1) p->blocks = 1;
+    G.run = (int)ceil_div(rows, p->blocks * G.teams);
+    if (G.run < 1) G.run = 1;
+    const int64_t edges = gate_rows > 1 ? p->blocks * G.teams * 4 * dim : 0;
+    p->bytes = (p->blocks * 4 * dim + edges) * (int64_t)sizeof(float);
+    return true;
+}
+
+#define MDQ_NORM_PICK(FN, XT, HT)                                                                  \
+    ((XT) == MDQ_F32 ? ((HT) == MDQ_F32 ? FN##_ff : FN##_fb) : ((HT) == MDQ_F32 ? FN##_bf : FN##_bb))
+
+bool vector_rows(const mdq_residual_norm_desc& d) {
+    const bool p = d.dim % kCols == 0 && aligned16(d.post_weight) && aligned16(d.post_bias) &&
+                   aligned16(d.pre_weight) && aligned16(d.pre_bias) && aligned16(d.gate);
+    return p && rows16(d.x, d.x_stride, d.x_dtype) &&
+           (d.h == nullptr || rows16(d.h, d.h_stride, d.h_dtype));
 }
 
 mdq_status check_norm(const mdq_residual_norm_desc& d, const char* what) {
@@ -227,7 +355,20 @@ mdq_status mdq_residual_norm(const mdq_residual_norm_desc* d, cudaStream_t strea
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm: null pointer");
     mdq_residual_norm_desc a = *d;
     if (a.pre_weight == nullptr) a.n = nullptr;
-    norm_forward<<<(unsigned)d->rows, kThreads, 0, stream>>>(a);
+    if (!aligned16(a.stats)) return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm: stats misaligned");
+    Teams G = {};
+    int cluster = 1;
+    if (plan_columns(a.dim, &cluster, &G)) {
+        const bool vec = vector_rows(a) && aligned16(a.x_new) && aligned16(a.n);
+        G.teams = cluster > 1 || G.threads > 128 ? 1 : 256 / G.threads;
+        // Two CTAs of 512 threads an SM, or as many smaller ones.
+        int64_t grid = ceil_div(a.rows, G.teams), most = 148 * (1024 / (G.threads * G.teams)) / cluster;
+        if (grid > most) grid = most;
+        return status_of(MDQ_NORM_PICK(forward, a.x_dtype, a.h_dtype)(a, G, (int)grid * cluster, cluster,
+                                                                      vec, stream),
+                         "residual norm");
+    }
+    norm_wide<<<(unsigned)d->rows, kThreads, 0, stream>>>(a);
     return launch_status("residual norm");
 }
 
@@ -236,7 +377,8 @@ mdq_status mdq_residual_norm_grad_workspace_bytes(int64_t rows, int64_t dim, int
     mdq_clear_error();
     if (bytes == nullptr || rows < 0 || dim < 1 || gate_rows < 1)
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: bad size");
-    *bytes = rows * 2 * (int64_t)sizeof(float);
+    GradPlan p;
+    *bytes = plan_grad(rows, dim, gate_rows, &p) ? p.bytes : rows * 2 * (int64_t)sizeof(float);
     return MDQ_OK;
 }
 
@@ -258,12 +400,37 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
     if (need > 0 && (g->workspace == nullptr || g->workspace_bytes < need))
         return mdq_fail(MDQ_ERR_INVALID_ARG, "workspace holds %lld bytes, %lld needed",
                         (long long)g->workspace_bytes, (long long)need);
-    float* means = static_cast<float*>(g->workspace);
-    if (g->f.rows > 0)
-        norm_backward_rows<<<(unsigned)g->f.rows, kThreads, 0, stream>>>(*g, means);
-    norm_backward_columns<<<(unsigned)((g->f.dim + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
-        *g, means);
-    return launch_status("residual norm grad");
+    if (!aligned16(g->workspace) || !aligned16(g->f.stats))
+        return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: workspace or stats misaligned");
+    GradPlan p;
+    if (!plan_grad(g->f.rows, g->f.dim, g->f.gate_rows, &p)) {
+        float* means = static_cast<float*>(g->workspace);
+        if (g->f.rows > 0)
+            norm_grad_wide<<<(unsigned)g->f.rows, kThreads, 0, stream>>>(*g, means);
+        norm_grad_wide_columns<<<(unsigned)ceil_div(g->f.dim, kThreads), kThreads, 0, stream>>>(*g, means);
+        return launch_status("residual norm grad");
+    }
+    const bool vec = vector_rows(g->f) && aligned16(g->grad_x) && aligned16(g->grad_h) &&
+                     (g->grad_new == nullptr || rows16(g->grad_new, g->grad_new_stride, g->f.x_dtype)) &&
+                     (g->grad_n == nullptr || rows16(g->grad_n, g->grad_n_stride, g->f.h_dtype));
+    const bool grouped = g->f.gate_rows > 1;
+    const bool full = g->f.kind == MDQ_NORM_LAYER || g->f.post_bias != nullptr || g->f.pre_bias != nullptr;
+    Partials W;
+    W.sums = static_cast<float*>(g->workspace);
+    W.edges = W.sums + p.blocks * 4 * g->f.dim;
+    st = status_of(MDQ_NORM_PICK(backward, g->f.x_dtype, g->f.h_dtype)(
+                       *g, p.G, W, (int)p.blocks * p.cluster, p.cluster, vec, full, grouped, stream),
+                   "residual norm grad");
+    if (st != MDQ_OK) return st;
+    const dim3 grid((unsigned)ceil_div(g->f.dim, 32), g->f.h != nullptr ? 2 : 1);
+    cudaError_t e = launch(norm_grad_sum, grid, 512, 0, stream, 1, true, *g, W, (int)p.blocks, (int)full,
+                           (int)grouped);
+    if (e == cudaSuccess && grouped && g->grad_gate != nullptr) {
+        const int64_t groups = g->f.gate_rows < 256 ? g->f.gate_rows : 256;
+        e = launch(norm_grad_gate, dim3((unsigned)ceil_div(g->f.dim, 256), (unsigned)groups), 256, 0,
+                   stream, 1, false, *g, W, p.G.run, (int)full);
+    }
+    return status_of(e, "residual norm grad");
 }
 
 }  // extern "C"

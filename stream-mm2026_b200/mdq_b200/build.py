@@ -26,7 +26,8 @@ SOURCES = ["mdq_step.cu", "mdq_stats.cu", "mdq_tiles_packed4.cu", "mdq_tiles_s8u
            "mdq_tiles_s16u16.cu", "mdq_tiles_s32u32.cu", "mdq_tiles_m8v4.cu",
            "mdq_blocks_packed4.cu", "mdq_blocks_s8u8.cu", "mdq_blocks_s16u16.cu",
            "mdq_blocks_s32u32.cu", "mdq_blocks_m8v4.cu", "mdq_staged_s8u8.cu", "mdq_staged_packed4.cu",
-           "mdq_fakequant.cu", "mdq_embed.cu", "mdq_norm.cu", "mdq_distill.cu"]
+           "mdq_fakequant.cu", "mdq_embed.cu", "mdq_norm.cu", "mdq_norm_ff.cu", "mdq_norm_fb.cu",
+           "mdq_norm_bb.cu", "mdq_norm_bf.cu", "mdq_distill.cu"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
