@@ -296,50 +296,6 @@ __device__ __forceinline__ void write_zeros(T* to, int64_t count, int tid, int t
         __stcs(reinterpret_cast<uint4*>(to + head) + u, make_uint4(0, 0, 0, 0));
 }
 
-// ------------------------------------------------------------------- copying
-
-__device__ __forceinline__ unsigned smem_at(const void* p) {
-    return (unsigned)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void bar_init(void* bar, int count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_at(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(void* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory");
-}
-
-// Whether the barrier's phase ended.  Phases last microseconds; the limit
-// (hundreds of milliseconds) only keeps a lost copy from hanging the GPU.
-__device__ __forceinline__ bool bar_wait(void* bar, unsigned parity) {
-    for (int i = 0; i < 1 << 22; ++i) {
-        unsigned done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(smem_at(bar)), "r"(parity) : "memory");
-        if (done) return true;
-    }
-    return false;
-}
-__device__ __forceinline__ unsigned long long read_once() {   // evict-first in L2
-    unsigned long long policy;
-    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    return policy;
-}
-// Arrives at the barrier with a copy of `bytes` (may be 0) that ends on it.
-__device__ __forceinline__ void copy_in(void* bar, void* to, const void* from, unsigned bytes,
-                                        unsigned long long policy) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes)
-                 : "memory");
-    if (bytes > 0)
-        asm volatile(
-            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-            " [%0], [%1], %2, [%3], %4;" ::"r"(smem_at(to)),
-            "l"(from), "r"(bytes), "r"(smem_at(bar)), "l"(policy)
-            : "memory");
-}
-
 // The 16-byte units a row of logits lies in, counted from the boundary at or
 // before its start; `lead` elements of the first precede the row.
 template <typename T>

@@ -272,28 +272,50 @@ __global__ void __launch_bounds__(256) norm_grad_gate(const __grid_constant__
 
 // ------------------------------------------------------------------ planning
 
-// Columns a CTA takes, its threads, and the CTAs of a row; false when the row is
-// too wide for a cluster.
-bool plan_columns(int64_t dim, int* cluster, Teams* G) {
+// Threads for `share` columns in `chunks` chunks of a thread.
+int threads_for(int64_t share, int chunks) { return (int)ceil_div(share, 32 * kCols * chunks) * 32; }
+
+// Columns a CTA takes and the CTAs of a row, with at most `chunks` chunks a
+// thread; false when the row is too wide for a cluster.
+bool plan_columns(int64_t dim, int chunks, int* cluster, Teams* G) {
+    const int64_t most = (int64_t)kTeam * kCols * chunks;
     *cluster = 1;
-    while (*cluster < kMaxCluster && dim > (int64_t)*cluster * kTeam * kCols) *cluster *= 2;
-    if (dim > (int64_t)*cluster * kTeam * kCols) return false;
+    while (*cluster < kMaxCluster && dim > *cluster * most) *cluster *= 2;
+    if (dim > *cluster * most) return false;
     G->share = (int)(ceil_div(ceil_div(dim, *cluster), kCols) * kCols);
-    G->threads = (int)ceil_div(G->share, kCols * 32) * 32;
+    return true;
+}
+
+// Forward: two chunks a thread for many rows above 256 columns, one for narrow
+// or few (as few threads as 512 allow), four where that is not enough.
+// 32768 bf16 rows of 768 / 128 columns: 48 / 18 us with two chunks, 108 / 15 with one.
+bool plan_forward(int64_t rows, int64_t dim, int* cluster, int* chunks, Teams* G, int* grid) {
+    if (!plan_columns(dim, 4, cluster, G)) return false;
+    *chunks = rows > 296 && G->share > 256 ? 2 : 1;
+    while (threads_for(G->share, *chunks) > kTeam) *chunks *= 2;
+    G->threads = threads_for(G->share, *chunks);
+    G->teams = *cluster > 1 || G->threads > 64 ? 1 : 128 / G->threads;
+    // 512 threads an SM, as their registers go.
+    const int64_t ctas = G->threads * G->teams >= kTeam ? 1 : kTeam / (G->threads * G->teams);
+    const int64_t need = ceil_div(rows, G->teams), most = 148 * ctas / *cluster;
+    *grid = (int)(need < most ? need : most);
+    G->run = (int)ceil_div(rows, (int64_t)*grid * G->teams);
+    *grid *= *cluster;
     return true;
 }
 
 // The backward pass's teams, their rows, and what the workspace holds.
 struct GradPlan {
     Teams G;
-    int cluster;
+    int cluster, chunks;
+    int stages;        // of the streaming kernel, 0: the other
+    size_t smem;
     int64_t blocks;    // clusters, each with a row of sums
     int64_t bytes;
 };
-bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, GradPlan* p) {
-    if (!plan_columns(dim, &p->cluster, &p->G)) return false;
+// Rows, sums and bytes once columns are given to threads.
+void plan_rows(int64_t rows, int64_t dim, int64_t gate_rows, GradPlan* p) {
     Teams& G = p->G;
-    G.teams = p->cluster > 1 ? 1 : kTeam / G.threads;
     // One CTA an SM (its registers end there), fewer where few rows would give
     // teams less than four, so that the sums over CTAs stay short.
     const int64_t most = 148 / p->cluster;
@@ -305,6 +327,38 @@ bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, GradPlan* p) {
     if (G.run < 1) G.run = 1;
     const int64_t edges = gate_rows > 1 ? p->blocks * G.teams * 4 * dim : 0;
     p->bytes = (p->blocks * 4 * dim + edges) * (int64_t)sizeof(float);
+}
+bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, bool full, GradPlan* p) {
+    // Four chunks where two sums of 16384 columns fit into shared memory.
+    const bool wide = !full && gate_rows == 1;
+    p->stages = 0;
+    p->smem = 0;
+    if (!plan_columns(dim, wide ? 4 : 2, &p->cluster, &p->G)) return false;
+    Teams& G = p->G;
+    p->chunks = 1;
+    while (threads_for(G.share, p->chunks) > kTeam) p->chunks *= 2;
+    G.threads = threads_for(G.share, p->chunks);
+    G.teams = p->cluster > 1 || p->chunks > 1 ? 1 : kTeam / G.threads;
+    plan_rows(rows, dim, gate_rows, p);
+    return true;
+}
+// The streaming kernel: two rows ahead at least, in 200 KB.
+bool plan_stream(int64_t rows, int64_t dim, int64_t gate_rows, int64_t row_bytes, bool full, GradPlan* p) {
+    p->chunks = 1;
+    // Above 8192 columns the steps between more than two CTAs take longer than the
+    // other kernel's rows (503 against 382 us for 4096 rows of 16384).
+    if (!plan_columns(dim, 1, &p->cluster, &p->G) || p->cluster > 2) return false;
+    Teams& G = p->G;
+    G.threads = threads_for(G.share, 1);
+    G.teams = p->cluster > 1 ? 1 : kTeam / G.threads;
+    const int64_t stage = row_bytes * G.share + 16, room = 200 * 1024;
+    while (G.teams > 1 && 3 * stage * G.teams > room) --G.teams;
+    int64_t stages = room / (stage * G.teams);
+    if (stages < 2) return false;
+    p->stages = stages < kMaxStages ? (int)stages : kMaxStages;
+    const int64_t sums = G.teams > 1 ? (full ? 4 : 2) * G.share * (int64_t)sizeof(float) : 0;
+    p->smem = (size_t)(p->stages * stage * G.teams > sums ? p->stages * stage * G.teams : sums);
+    plan_rows(rows, dim, gate_rows, p);
     return true;
 }
 
@@ -357,15 +411,12 @@ mdq_status mdq_residual_norm(const mdq_residual_norm_desc* d, cudaStream_t strea
     if (a.pre_weight == nullptr) a.n = nullptr;
     if (!aligned16(a.stats)) return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm: stats misaligned");
     Teams G = {};
-    int cluster = 1;
-    if (plan_columns(a.dim, &cluster, &G)) {
+    int cluster = 1, chunks = 1, grid = 1;
+    if (plan_forward(a.rows, a.dim, &cluster, &chunks, &G, &grid)) {
         const bool vec = vector_rows(a) && aligned16(a.x_new) && aligned16(a.n);
-        G.teams = cluster > 1 || G.threads > 128 ? 1 : 256 / G.threads;
-        // Two CTAs of 512 threads an SM, or as many smaller ones.
-        int64_t grid = ceil_div(a.rows, G.teams), most = 148 * (1024 / (G.threads * G.teams)) / cluster;
-        if (grid > most) grid = most;
-        return status_of(MDQ_NORM_PICK(forward, a.x_dtype, a.h_dtype)(a, G, (int)grid * cluster, cluster,
-                                                                      vec, stream),
+        const bool full = a.kind == MDQ_NORM_LAYER || a.post_bias != nullptr || a.pre_bias != nullptr;
+        return status_of(MDQ_NORM_PICK(forward, a.x_dtype, a.h_dtype)(a, G, chunks, grid, cluster, vec,
+                                                                      full, stream),
                          "residual norm");
     }
     norm_wide<<<(unsigned)d->rows, kThreads, 0, stream>>>(a);
@@ -377,8 +428,15 @@ mdq_status mdq_residual_norm_grad_workspace_bytes(int64_t rows, int64_t dim, int
     mdq_clear_error();
     if (bytes == nullptr || rows < 0 || dim < 1 || gate_rows < 1)
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: bad size");
-    GradPlan p;
-    *bytes = plan_grad(rows, dim, gate_rows, &p) ? p.bytes : rows * 2 * (int64_t)sizeof(float);
+    // Enough for either kind of norm and all types.
+    *bytes = rows * 2 * (int64_t)sizeof(float);
+    for (int full = 0; full < 2; ++full)
+        for (int row_bytes = 0; row_bytes <= 16; row_bytes += row_bytes < 8 ? 8 : 4) {
+            GradPlan p;
+            const bool ok = row_bytes == 0 ? plan_grad(rows, dim, gate_rows, full, &p)
+                                           : plan_stream(rows, dim, gate_rows, row_bytes, full, &p);
+            if (ok && p.bytes > *bytes) *bytes = p.bytes;
+        }
     return MDQ_OK;
 }
 
@@ -402,8 +460,10 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
                         (long long)g->workspace_bytes, (long long)need);
     if (!aligned16(g->workspace) || !aligned16(g->f.stats))
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: workspace or stats misaligned");
+    const bool grouped = g->f.gate_rows > 1;
+    const bool full = g->f.kind == MDQ_NORM_LAYER || g->f.post_bias != nullptr || g->f.pre_bias != nullptr;
     GradPlan p;
-    if (!plan_grad(g->f.rows, g->f.dim, g->f.gate_rows, &p)) {
+    if (!plan_grad(g->f.rows, g->f.dim, g->f.gate_rows, full, &p)) {
         float* means = static_cast<float*>(g->workspace);
         if (g->f.rows > 0)
             norm_grad_wide<<<(unsigned)g->f.rows, kThreads, 0, stream>>>(*g, means);
@@ -413,17 +473,21 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
     const bool vec = vector_rows(g->f) && aligned16(g->grad_x) && aligned16(g->grad_h) &&
                      (g->grad_new == nullptr || rows16(g->grad_new, g->grad_new_stride, g->f.x_dtype)) &&
                      (g->grad_n == nullptr || rows16(g->grad_n, g->grad_n_stride, g->f.h_dtype));
-    const bool grouped = g->f.gate_rows > 1;
-    const bool full = g->f.kind == MDQ_NORM_LAYER || g->f.post_bias != nullptr || g->f.pre_bias != nullptr;
+    const int row_bytes = 2 * (int)(type_size(g->f.x_dtype) + type_size(g->f.h_dtype));
+    GradPlan q;
+    if (vec && plan_stream(g->f.rows, g->f.dim, g->f.gate_rows, row_bytes, full, &q)) p = q;
     Partials W;
     W.sums = static_cast<float*>(g->workspace);
     W.edges = W.sums + p.blocks * 4 * g->f.dim;
-    st = status_of(MDQ_NORM_PICK(backward, g->f.x_dtype, g->f.h_dtype)(
-                       *g, p.G, W, (int)p.blocks * p.cluster, p.cluster, vec, full, grouped, stream),
+    const int grid = (int)p.blocks * p.cluster;
+    st = status_of(p.stages > 0 ? MDQ_NORM_PICK(stream, g->f.x_dtype, g->f.h_dtype)(
+                                      *g, p.G, W, p.stages, p.smem, grid, p.cluster, full, grouped, stream)
+                                : MDQ_NORM_PICK(backward, g->f.x_dtype, g->f.h_dtype)(
+                                      *g, p.G, W, p.chunks, grid, p.cluster, vec, full, grouped, stream),
                    "residual norm grad");
     if (st != MDQ_OK) return st;
-    const dim3 grid((unsigned)ceil_div(g->f.dim, 32), g->f.h != nullptr ? 2 : 1);
-    cudaError_t e = launch(norm_grad_sum, grid, 512, 0, stream, 1, true, *g, W, (int)p.blocks, (int)full,
+    const dim3 columns((unsigned)ceil_div(g->f.dim, 32), g->f.h != nullptr ? 2 : 1);
+    cudaError_t e = launch(norm_grad_sum, columns, 512, 0, stream, 1, true, *g, W, (int)p.blocks, (int)full,
                            (int)grouped);
     if (e == cudaSuccess && grouped && g->grad_gate != nullptr) {
         const int64_t groups = g->f.gate_rows < 256 ? g->f.gate_rows : 256;

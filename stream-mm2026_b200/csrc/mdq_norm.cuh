@@ -4,18 +4,18 @@
 //
 // Both passes are bound by memory: forward reads x and h and writes x_new and n,
 // backward reads x, h and the two gradients and writes two.  A row is held in
-// registers, 8 columns a thread, by a team of up to 512 threads; rows of more
-// than 4096 columns by a cluster of CTAs that exchange their sums through
-// distributed shared memory.  A team goes through rows one after another and
-// loads the next while it works on the present one; parameters come from the L1
-// cache at the place of use.  The backward pass keeps the parameters' gradients
-// of its rows in registers and leaves one partial sum for each CTA, which a
-// second kernel adds in a fixed order.
+// registers, up to 32 columns a thread, by a team of up to 512 threads; rows that
+// are wider by a cluster of CTAs that exchange their sums through distributed
+// shared memory.  Parameters come from the L1 cache at the place of use.  The
+// backward pass keeps the parameters' gradients of a team's rows on the chip and
+// leaves one partial sum for each CTA, which a second kernel adds in a fixed
+// order.
 #pragma once
 
 #include "mdq_ops.cuh"
 
 #include <cooperative_groups.h>
+#include <math_constants.h>
 
 namespace mdq_norm {
 
@@ -23,7 +23,7 @@ using namespace mdq_ops;
 namespace cg = cooperative_groups;
 
 constexpr int kTeam = 512;          // threads of a team at most
-constexpr int kCols = 8;            // columns of a thread
+constexpr int kCols = 8;            // columns of a thread's chunk
 constexpr int kMaxCluster = 8;
 
 // How rows are given to threads.
@@ -31,17 +31,40 @@ struct Teams {
     int threads;    // of a team, a multiple of 32
     int teams;      // of a CTA (1 in a cluster)
     int share;      // columns of a CTA
-    int run;        // rows of a team, consecutive (backward)
+    int run;        // rows of a team, consecutive
 };
 
-// The columns of a thread: 8 consecutive ones on 16-byte boundaries (VECTOR), or
-// `step` apart.
+// The columns of one chunk of a thread: 8 consecutive ones on 16-byte boundaries
+// (VECTOR), or `step` apart.
 template <bool VECTOR>
 struct Cols {
     int first, step, end;
     __device__ __forceinline__ int at(int k) const { return first + (VECTOR ? k : k * step); }
     __device__ __forceinline__ bool has(int k) const { return VECTOR ? first < end : at(k) < end; }
+    // The thread's chunk i.
+    __device__ __forceinline__ Cols chunk(int i) const { return {first + i * step * 8, step, end}; }
 };
+
+// Eight values in pairs: products, sums and fused products of a pair are one
+// instruction each, which about halves what the kernels issue.
+typedef float2 F8[4];
+__device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ void fill(F8& v, float x) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = both(x);
+}
+__device__ __forceinline__ float value(const F8& v, int k) { return k & 1 ? v[k >> 1].y : v[k >> 1].x; }
+__device__ __forceinline__ void set(F8& v, int k, float x) { (k & 1 ? v[k >> 1].y : v[k >> 1].x) = x; }
+
+__device__ __forceinline__ void unpack(uint4 w, F8& v) {
+    const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        v[j] = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+}
 
 // Eight values as they were loaded, 0 outside of the row.
 template <typename T, bool VECTOR>
@@ -52,7 +75,7 @@ struct Raw<__nv_bfloat16, true> {
     __device__ __forceinline__ void load(const __nv_bfloat16* row, const Cols<true>& c) {
         if (c.has(0)) a = __ldcs(reinterpret_cast<const uint4*>(row + c.first));
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const { Vec<__nv_bfloat16>::unpack(a, v); }
+    __device__ __forceinline__ void get(F8& v) const { unpack(a, v); }
 };
 template <>
 struct Raw<float, true> {
@@ -63,9 +86,11 @@ struct Raw<float, true> {
             b = __ldcs(reinterpret_cast<const float4*>(row + c.first) + 1);
         }
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    __device__ __forceinline__ void get(F8& v) const {
+        v[0] = make_float2(a.x, a.y);
+        v[1] = make_float2(a.z, a.w);
+        v[2] = make_float2(b.x, b.y);
+        v[3] = make_float2(b.z, b.w);
     }
 };
 template <typename T>
@@ -80,48 +105,82 @@ struct Raw<T, false> {
         for (int k = 0; k < 8; ++k)
             if (c.has(k)) a[k] = row[c.at(k)];
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
+    __device__ __forceinline__ void get(F8& v) const {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = to_f(a[k]);
+        for (int k = 0; k < 8; ++k) set(v, k, to_f(a[k]));
     }
 };
 
 template <typename T, bool VECTOR>
-__device__ __forceinline__ void store(T* row, const Cols<VECTOR>& c, const float (&v)[8]) {
+__device__ __forceinline__ void store(T* row, const Cols<VECTOR>& c, const F8& v) {
     if constexpr (!VECTOR) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (c.has(k)) row[c.at(k)] = from_f<T>(v[k]);
+            if (c.has(k)) row[c.at(k)] = from_f<T>(value(v, k));
     } else if (c.has(0)) {
         if constexpr (sizeof(T) == 2) {
-            *reinterpret_cast<uint4*>(row + c.first) = Vec<T>::pack(v);
+            *reinterpret_cast<uint4*>(row + c.first) =
+                make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y),
+                           pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
         } else {
-            reinterpret_cast<float4*>(row + c.first)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(row + c.first)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            reinterpret_cast<float4*>(row + c.first)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            reinterpret_cast<float4*>(row + c.first)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
         }
     }
 }
 
-// Parameters of the thread's columns; `none` without an array.
+// Parameters of a chunk: `none` without an array, 0 outside of the row.
 template <bool VECTOR>
 __device__ __forceinline__ void parameters(const void* p, bool bf16, const Cols<VECTOR>& c, float none,
-                                           float (&v)[8]) {
-    if (p == nullptr || !c.has(0)) {
+                                           F8& v) {
+    if (p == nullptr || (VECTOR && !c.has(0))) {
+        fill(v, c.has(0) ? none : 0.0f);
+        if constexpr (!VECTOR)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = none;
+            for (int k = 0; k < 8; ++k)
+                if (!c.has(k)) set(v, k, 0.0f);
     } else if constexpr (VECTOR) {
         if (bf16) {
-            Vec<__nv_bfloat16>::unpack(
-                __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + c.first)), v);
+            unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + c.first)), v);
         } else {
             const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + c.first);
             const float4 a = __ldg(q), b = __ldg(q + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            v[0] = make_float2(a.x, a.y);
+            v[1] = make_float2(a.z, a.w);
+            v[2] = make_float2(b.x, b.y);
+            v[3] = make_float2(b.z, b.w);
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = c.has(k) ? load_any(p, bf16, c.at(k)) : none;
+        for (int k = 0; k < 8; ++k) set(v, k, c.has(k) ? load_any(p, bf16, c.at(k)) : 0.0f);
+    }
+}
+// p = gate * weight and b = gate * bias (FULL), both 0 outside of the row.
+template <bool FULL, bool VECTOR>
+__device__ __forceinline__ void post_parameters(const mdq_residual_norm_desc& d, const void* gate, bool pb,
+                                                const Cols<VECTOR>& c, F8& p, F8& b) {
+    F8 g;
+    parameters(d.post_weight, pb, c, 1.0f, p);
+    if (FULL) parameters(d.post_bias, pb, c, 0.0f, b);
+    if (gate == nullptr) return;
+    parameters(gate, pb, c, 1.0f, g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        p[j] = mul(p[j], g[j]);
+        if (FULL) b[j] = mul(b[j], g[j]);
+    }
+}
+// The values less `mean` inside of the row; outside they are 0 and stay 0.
+template <bool VECTOR>
+__device__ __forceinline__ void less(F8& v, const Cols<VECTOR>& c, float mean) {
+    if constexpr (VECTOR) {
+        const float2 m = both(c.has(0) ? -mean : 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = add(v[j], m);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c.has(k)) set(v, k, value(v, k) - mean);
     }
 }
 
@@ -130,33 +189,55 @@ constexpr int kSlots = kMaxCluster * kTeam / 32;
 
 // Sums over a team, and over the cluster where that is larger.
 struct Reducer {
-    float2 (*slots)[kSlots];   // [2][CTAs x warps], from `base` on this team's
+    float* slots;     // [2][values x warps x CTAs]; this team's part begins at warp `base`
+    int size;         // floats of one of the two
     int base, team, warp, warps, lane, parity, ctas, rank;
 
-    template <int NV>
-    __device__ __forceinline__ void sum(float (&v)[NV]) {
+    // The sums of 2^LOG values, given to every thread.  Within a warp lanes hand
+    // half of their values over in each of the first LOG steps, so that the
+    // shuffles grow with the number of values and not with five times that.
+    template <int LOG>
+    __device__ __forceinline__ void sum(float (&v)[1 << LOG]) {
+        constexpr int NV = 1 << LOG, kGroup = 32 >> LOG;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) v[k] = warp_sum(v[k]);
-        if (warps == 1 && ctas == 1) return;
-        const float2 mine = make_float2(v[0], NV > 1 ? v[NV - 1] : 0.0f);
-        float2* buf = slots[parity] + base;
-        parity ^= 1;   // the other buffer is read until every thread is past the next barrier
-        if (ctas == 1) {
-            if (lane == 0) buf[warp] = mine;
-            asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(warps * 32) : "memory");
-        } else {
-            cg::cluster_group cluster = cg::this_cluster();
-            if (lane < ctas) cluster.map_shared_rank(buf, lane)[rank * warps + warp] = mine;
-            cluster.sync();
+        for (int s = 0; s < LOG; ++s) {
+            const bool upper = lane & 16 >> s;
+#pragma unroll
+            for (int j = 0; j < NV >> (s + 1); ++j) {
+                float& high = v[j + (NV >> (s + 1))];
+                const float keep = upper ? high : v[j], give = upper ? v[j] : high;
+                v[j] = keep + __shfl_xor_sync(0xffffffffu, give, 16 >> s);
+            }
         }
-        float2 s = make_float2(0.0f, 0.0f);
-        for (int i = lane; i < ctas * warps; i += 32) {
-            const float2 p = buf[i];
-            s.x += p.x;
-            s.y += p.y;
+        float r = v[0];   // of value lane / kGroup
+#pragma unroll
+        for (int o = kGroup / 2; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+        if (warps > 1 || ctas > 1) {
+            float* buf = slots + parity * size + base * NV;
+            parity ^= 1;   // the other buffer is read until every thread is past the next barrier
+            const int value = lane / kGroup, sub = lane % kGroup;
+            if (ctas == 1) {
+                if (sub == 0) buf[warp * NV + value] = r;
+                asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(warps * 32) : "memory");
+            } else {
+                cg::cluster_group cluster = cg::this_cluster();
+                for (int k = sub; k < ctas; k += kGroup)
+                    cluster.map_shared_rank(buf, k)[(rank * warps + warp) * NV + value] = r;
+                cluster.sync();
+            }
+            r = 0.0f;
+            if (ctas == 1) {   // 16 warps at most
+#pragma unroll
+                for (int k = 0; k < 16; k += kGroup)
+                    if (k + sub < warps) r += buf[(k + sub) * NV + value];
+            } else {
+                for (int k = sub; k < ctas * warps; k += kGroup) r += buf[k * NV + value];
+            }
+#pragma unroll
+            for (int o = kGroup / 2; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
         }
-        v[0] = warp_sum(s.x);
-        if (NV > 1) v[NV - 1] = warp_sum(s.y);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = __shfl_sync(0xffffffffu, r, j * kGroup);
     }
 };
 
@@ -167,14 +248,14 @@ struct Place {
     Cols<VECTOR> cols;
     int t, team;
     int64_t index, count;   // of the team among all
-    __device__ __forceinline__ Place(const Teams& G, int dim,
-                                     float2 (*slots)[kSlots]) {
+    __device__ __forceinline__ Place(const Teams& G, int dim, float* slots, int size) {
         team = threadIdx.x / G.threads;
         t = threadIdx.x - team * G.threads;
         cg::cluster_group cluster = cg::this_cluster();
         R.ctas = (int)cluster.num_blocks();
         R.rank = (int)cluster.block_rank();
         R.slots = slots;
+        R.size = size;
         R.base = team * (G.threads >> 5);
         R.team = team;
         R.warp = t >> 5;
@@ -190,91 +271,156 @@ struct Place {
     }
 };
 
-// Mean and 1 / deviation of a row (mean 0 without `layer`), the values with
-// their mean removed in `c`; places outside of the row become 0.
-template <bool VECTOR>
-__device__ __forceinline__ float2 statistics(Reducer& R, const Cols<VECTOR>& cols, const float (&v)[8],
-                                             float (&c)[8], bool layer, float inv, float eps) {
+// Mean and 1 / deviation of a row (mean 0 without `layer`); its values lose
+// their mean.
+template <int I, bool VECTOR>
+__device__ __forceinline__ float2 statistics(Reducer& R, const Cols<VECTOR>& cols, F8 (&v)[I],
+                                             bool layer, float inv, float eps) {
     float mean = 0.0f;
     if (layer) {
-        float s[1] = {0.0f};
+        float2 t = both(0.0f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s[0] += v[k];
-        R.sum(s);
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t = add(t, v[i][j]);
+        float s[1] = {t.x + t.y};
+        R.sum<0>(s);
         mean = s[0] * inv;
-    }
-    float q[1] = {0.0f};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        c[k] = cols.has(k) ? v[k] - mean : 0.0f;
-        q[0] = fmaf(c[k], c[k], q[0]);
+        for (int i = 0; i < I; ++i) less(v[i], cols.chunk(i), mean);
     }
-    R.sum(q);
+    float2 t = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t = fma(v[i][j], v[i][j], t);
+    float q[1] = {t.x + t.y};
+    R.sum<0>(q);
     return make_float2(mean, 1.0f / sqrtf(fmaf(q[0], inv, eps)));
 }
 
-template <typename XT, typename HT, bool VECTOR>
-__global__ void __launch_bounds__(kTeam, 2) norm_rows(const __grid_constant__ mdq_residual_norm_desc d,
+// I chunks of 8 columns a thread.  With one or two, the parameters stay in
+// registers over a team's rows and the next row is loaded ahead; with four (rows
+// above 8192 columns) neither fits, and a row is long enough to fill the time.
+// FULL: layer norm or biases.
+template <typename XT, typename HT, bool VECTOR, int I, bool FULL>
+__global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ mdq_residual_norm_desc d,
                                                       const __grid_constant__ Teams G) {
-    __shared__ float2 slots[2][kSlots];
-    Place<VECTOR> P(G, (int)d.dim, slots);
+    __shared__ float slots[2 * kSlots];
+    Place<VECTOR> P(G, (int)d.dim, slots, kSlots);
     const Cols<VECTOR>& cols = P.cols;
     if (P.R.ctas > 1) cg::this_cluster().sync();   // all run before their memory is written to
-    const bool layer = d.kind == MDQ_NORM_LAYER, pb = d.param_dtype == MDQ_BF16;
+    const bool layer = FULL && d.kind == MDQ_NORM_LAYER, pb = d.param_dtype == MDQ_BF16;
     const float inv = 1.0f / (float)d.dim;
     const XT* x = static_cast<const XT*>(d.x);
     const HT* h = static_cast<const HT*>(d.h);
     const int64_t per = d.rows / d.gate_rows;
-    Raw<XT, VECTOR> nx;
-    Raw<HT, VECTOR> nh;
-    const auto fetch = [&](int64_t r) {
-        nx.load(x + r * d.x_stride, cols);
-        if (h != nullptr) nh.load(h + r * d.h_stride, cols);
+    const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
+    constexpr bool kKeep = I <= 2;
+    F8 kp[kKeep ? I : 1], kb[kKeep && FULL ? I : 1], kw[kKeep ? I : 1], kc[kKeep && FULL ? I : 1];
+    if constexpr (kKeep) {
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            parameters(d.pre_weight, pb, cols.chunk(i), 1.0f, kw[i]);
+            if (FULL) parameters(d.pre_bias, pb, cols.chunk(i), 0.0f, kc[FULL ? i : 0]);
+        }
+    }
+    Raw<XT, VECTOR> nx[I];
+    Raw<HT, VECTOR> nh[I];
+    const XT* xr = x + r0 * d.x_stride;
+    const HT* hr = h + r0 * d.h_stride;
+    const auto fetch = [&] {   // the next row
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            if (h != nullptr) nh[i].load(hr, cols.chunk(i));
+            nx[i].load(xr, cols.chunk(i));
+        }
+        xr += d.x_stride;
+        hr += d.h_stride;
     };
-    if (P.index < d.rows) fetch(P.index);
-    for (int64_t r = P.index; r < d.rows; r += P.count) {
-        float v[8], c[8];
+    XT* xo = static_cast<XT*>(d.x_new) + r0 * d.dim;
+    HT* no = static_cast<HT*>(d.n) + r0 * d.dim;
+    if (kKeep && r0 < r1) fetch();
+    int64_t turn = r0;   // the row at which another row of the gate begins
+    for (int64_t r = r0; r < r1; ++r, xo += d.dim, no += d.dim) {
+        const void* gate = d.gate;
+        if (gate != nullptr && d.gate_rows > 1 && (!kKeep || r == turn))
+            gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
+        if (kKeep && r == turn) {
+            if (h != nullptr)
+#pragma unroll
+                for (int i = 0; i < I; ++i)
+                    post_parameters<FULL>(d, gate, pb, cols.chunk(i), kp[kKeep ? i : 0],
+                                          kb[kKeep && FULL ? i : 0]);
+            turn = d.gate_rows > 1 ? (r / per + 1) * per : r1;
+        }
+        F8 v[I];
+        Raw<XT, VECTOR> rx[I];
         float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const Raw<XT, VECTOR> rx = nx;
-        const Raw<HT, VECTOR> rh = nh;
-        if (r + P.count < d.rows) fetch(r + P.count);
+        if (!kKeep) fetch();
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            rx[i] = nx[i];
+            nh[i].get(v[i]);
+        }
+        if (kKeep && r + 1 < r1) fetch();
         if (h != nullptr) {
-            rh.get(v);
-            const float2 s = statistics(P.R, cols, v, c, layer, inv, d.eps);
+            const float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
             st.x = s.x;
             st.y = s.y;
-            float w[8];
-            parameters(d.post_weight, pb, cols, 1.0f, w);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] *= s.y * w[k];
-            if (d.post_bias != nullptr) {
-                parameters(d.post_bias, pb, cols, 0.0f, w);
+            for (int i = 0; i < I; ++i) {
+                const Cols<VECTOR> c = cols.chunk(i);
+                F8 p, b, xv;
+                if constexpr (kKeep) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) c[k] += w[k];
+                    for (int j = 0; j < 4; ++j) {
+                        p[j] = kp[i][j];
+                        b[j] = kb[FULL ? i : 0][j];
+                    }
+                } else {
+                    post_parameters<FULL>(d, gate, pb, c, p, b);
+                }
+                rx[i].get(xv);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[i][j] = mul(v[i][j], both(s.y));
+                    if (FULL) v[i][j] = fma(v[i][j], p[j], b[j]);
+                    else v[i][j] = mul(v[i][j], p[j]);
+                    v[i][j] = fma(both(d.residual_scale), xv[j], v[i][j]);
+                }
+                store(xo, c, v[i]);
             }
-            if (d.gate != nullptr) {
-                const int64_t row = d.gate_rows == 1 ? 0 : r / per;
-                parameters(static_cast<const char*>(d.gate) + row * d.dim * (pb ? 2 : 4), pb, cols, 1.0f, w);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) c[k] *= w[k];
-            }
-            rx.get(v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = fmaf(d.residual_scale, v[k], c[k]);
-            store(static_cast<XT*>(d.x_new) + r * d.dim, cols, v);
         } else {
-            rx.get(v);
+#pragma unroll
+            for (int i = 0; i < I; ++i) rx[i].get(v[i]);
         }
         if (d.n != nullptr) {
-            const float2 s = statistics(P.R, cols, v, c, layer, inv, d.eps);
+            const float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
             st.z = s.x;
             st.w = s.y;
-            float w[8], b[8];
-            parameters(d.pre_weight, pb, cols, 1.0f, w);
-            parameters(d.pre_bias, pb, cols, 0.0f, b);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = fmaf(c[k] * s.y, w[k], b[k]);
-            store(static_cast<HT*>(d.n) + r * d.dim, cols, c);
+            for (int i = 0; i < I; ++i) {
+                const Cols<VECTOR> c = cols.chunk(i);
+                F8 w, b;
+                if constexpr (kKeep) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        w[j] = kw[i][j];
+                        b[j] = kc[FULL ? i : 0][j];
+                    }
+                } else {
+                    parameters(d.pre_weight, pb, c, 1.0f, w);
+                    if (FULL) parameters(d.pre_bias, pb, c, 0.0f, b);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[i][j] = mul(v[i][j], both(s.y));
+                    if (FULL) v[i][j] = fma(v[i][j], w[j], b[j]);
+                    else v[i][j] = mul(v[i][j], w[j]);
+                }
+                store(no, c, v[i]);
+            }
         }
         if (d.stats != nullptr && P.t == 0 && P.R.rank == 0)
             reinterpret_cast<float4*>(d.stats)[r] = st;
@@ -284,28 +430,117 @@ __global__ void __launch_bounds__(kTeam, 2) norm_rows(const __grid_constant__ md
 
 // ------------------------------------------------------------------ backward
 
-// Sums of the rows of one CTA, [kinds][dim] each, and the gate's sums of runs
-// that begin or end within a CTA's rows (GROUPED).
+// Sums of the rows of one CTA, [kinds][dim] each.
 enum { kPre = 0, kPost = 1, kPreBias = 2, kPostBias = 3 };   // of dn xh, t hh (times the gate), dn, t
 
-// Rows of the workspace: [block][4][dim], then (GROUPED) [team][2 edges][2][dim].
+// Rows of the workspace: [block][4][dim], then (GROUPED) [team][2 edges][2][dim]:
+// the gate's sums of runs that begin or end within a team's rows.
 struct Partials {
     float* sums;
     float* edges;
 };
 
+// What one chunk of a row holds.
+template <typename XT, typename HT, bool VECTOR>
+struct GradRaw {
+    Raw<XT, VECTOR> x, gx;
+    Raw<HT, VECTOR> h, gn;
+};
+
+// A group's sums of t hh and t leave the registers: the gate's gradient, or the
+// team's part of it, and their share of the parameters' gradients.
+template <bool VECTOR, bool FULL, int G, int A>
+__device__ __forceinline__ void end_group(const mdq_residual_norm_grad_desc& g, const void* gate, bool pb,
+                                          const Cols<VECTOR>& c, int64_t k0, float* edge, F8 (&group)[G],
+                                          F8 (&acc)[A]) {
+    const int64_t dim = g.f.dim;
+    F8 w, w1, b1;
+    parameters(gate, pb, c, 1.0f, w);
+    parameters(g.f.post_weight, pb, c, 1.0f, w1);
+    parameters(FULL ? g.f.post_bias : nullptr, pb, c, 0.0f, b1);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (!c.has(k)) continue;
+        const float sum = value(group[0], k), sum_b = value(group[G - 1], k);
+        set(acc[kPost], k, fmaf(value(w, k), sum, value(acc[kPost], k)));
+        if (FULL) set(acc[A - 1], k, fmaf(value(w, k), sum_b, value(acc[A - 1], k)));
+        if (edge != nullptr) {
+            edge[c.at(k)] = sum;
+            edge[dim + c.at(k)] = sum_b;
+        } else if (g.grad_gate != nullptr) {
+            store_any(g.grad_gate, pb, k0 * dim + c.at(k), fmaf(value(w1, k), sum, value(b1, k) * sum_b));
+        }
+    }
+    fill(group[0], 0.0f);
+    fill(group[G - 1], 0.0f);
+}
+
+// The CTA's sums, its teams adding theirs in turn in `shared` ([KINDS][share]).
+template <bool VECTOR, int KINDS>
+__device__ __forceinline__ void end_sums(const Place<VECTOR>& P, const Teams& G, const Partials& W, int dim,
+                                         float* shared, const F8 (&acc)[KINDS]) {
+    const int c0 = P.R.rank * G.share;
+    float* out = W.sums + (int64_t)(blockIdx.x / P.R.ctas) * 4 * dim;
+    for (int i = 0; i < G.teams; ++i) {
+        if (i > 0) __syncthreads();
+        if (P.team != i) continue;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (!P.cols.has(k)) continue;
+#pragma unroll
+            for (int j = 0; j < KINDS; ++j) {
+                float* q = shared + j * G.share + P.cols.at(k) - c0;
+                const float v = i > 0 ? *q + value(acc[j], k) : value(acc[j], k);
+                if (i + 1 < G.teams) *q = v;
+                else out[(int64_t)j * dim + P.cols.at(k)] = v;
+            }
+        }
+    }
+}
+
+// Eight values of a row in shared memory.
+template <typename T>
+__device__ __forceinline__ void from_shared(const char* row, int at, F8& v) {
+    const T* p = reinterpret_cast<const T*>(row) + at;
+    if constexpr (sizeof(T) == 2) {
+        unpack(*reinterpret_cast<const uint4*>(p), v);
+    } else {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = make_float2(a.x, a.y);
+        v[1] = make_float2(a.z, a.w);
+        v[2] = make_float2(b.x, b.y);
+        v[3] = make_float2(b.z, b.w);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void to_shared(char* row, int at, const F8& v) {
+    T* p = reinterpret_cast<T*>(row) + at;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) p[k] = from_f<T>(value(v, k));
+}
+constexpr int kMaxStages = 6;
+
+// With q = g w1 hh and p = g w1, the gradient u = t p of the normalised block has
+//   sum u hh = sum dx q + r2 (sum e q - m0 sum q - m1 sum xh q)
+// (and sum u the same with p for q), so that all sums of a row are taken in one
+// step, from which m1 = mean(e xh), m0 = mean(e) and the means of u follow.
+//
 // FULL: a mean is removed or a bias is there, so sums without the normalised
-// value are needed as well.  GROUPED: the gate differs between rows; its sums
-// leave the registers at the end of every group, weighted into the others.
-template <typename XT, typename HT, bool VECTOR, bool FULL, bool GROUPED>
+// value are needed as well.  GROUPED: the gate differs between rows; its sums go
+// out at the end of every group, weighted into the others.  With one chunk a
+// thread the parameters' gradients stay in registers; with more (rows above 4096
+// columns) they are in shared memory, each value of one thread.
+template <typename XT, typename HT, bool VECTOR, int I, bool FULL, bool GROUPED>
 __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant__
                                                            mdq_residual_norm_grad_desc g,
                                                            const __grid_constant__ Teams G,
                                                            const __grid_constant__ Partials W) {
-    __shared__ float2 slots[2][kSlots];
-    extern __shared__ float shared[];   // [2 or 4][share] where a CTA has several teams
+    constexpr int kLog = FULL ? 4 : 2, kKinds = FULL ? 4 : 2;
+    constexpr bool kRegs = I == 1;
+    __shared__ float slots[2 * kSlots * (1 << kLog)];
+    extern __shared__ __align__(16) float shared[];   // [kinds][share] (several teams, or I > 1)
     const mdq_residual_norm_desc& d = g.f;
-    Place<VECTOR> P(G, (int)d.dim, slots);
+    Place<VECTOR> P(G, (int)d.dim, slots, kSlots << kLog);
     const Cols<VECTOR>& cols = P.cols;
     if (P.R.ctas > 1) cg::this_cluster().sync();
     const bool layer = FULL && d.kind == MDQ_NORM_LAYER, pb = d.param_dtype == MDQ_BF16;
@@ -316,196 +551,571 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
     const HT* gn = static_cast<const HT*>(g.grad_n);
     const int64_t per = d.rows / d.gate_rows;
     const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
+    const int c0 = P.R.rank * G.share;
 
-    float pre[8] = {}, post[8] = {}, pre_b[FULL ? 8 : 1] = {}, post_b[FULL ? 8 : 1] = {};
-    float all[GROUPED ? 8 : 1] = {}, all_b[GROUPED && FULL ? 8 : 1] = {};
-    // fp32 rows fill the registers: they are not loaded ahead.
-    constexpr bool kAhead = sizeof(XT) + sizeof(HT) <= 6;
-    Raw<XT, VECTOR> nx, ngx;
-    Raw<HT, VECTOR> nh, ngn;
-    float4 nst = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const auto fetch = [&](int64_t r) {
-        nx.load(x + r * d.x_stride, cols);
-        if (h != nullptr) nh.load(h + r * d.h_stride, cols);
-        if (gn != nullptr) ngn.load(gn + r * g.grad_n_stride, cols);
-        if (gx != nullptr) ngx.load(gx + r * g.grad_new_stride, cols);
-        nst = __ldg(reinterpret_cast<const float4*>(d.stats) + r);
+    // The parameters' gradients; with GROUPED the sums of the present group apart.
+    F8 acc[kRegs ? kKinds : 1], group[GROUPED && kRegs ? 2 : 1];
+#pragma unroll
+    for (int j = 0; j < (kRegs ? kKinds : 1); ++j) fill(acc[j], 0.0f);
+#pragma unroll
+    for (int j = 0; j < (GROUPED && kRegs ? 2 : 1); ++j) fill(group[j], 0.0f);
+    const auto place_of = [&](int kind, const Cols<VECTOR>& c, int k) {
+        return shared + kind * G.share + c.at(k) - c0;
     };
-    if (kAhead && r0 < r1) fetch(r0);
-    // The rows of every CTA of a cluster are the same, so all take part in its sums.
-    for (int64_t r = r0; r < r1; ++r) {
-        if (!kAhead) fetch(r);
-        const Raw<XT, VECTOR> rx = nx, rgx = ngx;
-        const Raw<HT, VECTOR> rh = nh, rgn = ngn;
-        const float4 st = nst;
-        if (kAhead && r + 1 < r1) fetch(r + 1);
-        const void* gate = d.gate;
-        if (GROUPED) gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
-
-        float t[8], hh[8], w[8], v[8];
-        if (h != nullptr) {
-            rh.get(hh);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) hh[k] = cols.has(k) ? (hh[k] - st.x) * st.y : 0.0f;
-        }
-        rgx.get(t);
-        if (gn != nullptr) {
-            // x_new and its normalised value, as the forward pass had them
-            float xh[8], e[8];
-            rx.get(xh);
-            if (h != nullptr) {
-                parameters(d.post_weight, pb, cols, 1.0f, w);
-                parameters(FULL ? d.post_bias : nullptr, pb, cols, 0.0f, v);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = fmaf(hh[k], w[k], v[k]);
-                parameters(gate, pb, cols, 1.0f, w);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) xh[k] = fmaf(d.residual_scale, xh[k], v[k] * w[k]);
-            }
-            rgn.get(e);
-            parameters(d.pre_weight, pb, cols, 1.0f, w);
-            float s[FULL ? 2 : 1] = {};
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                xh[k] = cols.has(k) ? (xh[k] - st.z) * st.w : 0.0f;
-                pre[k] = fmaf(e[k], xh[k], pre[k]);
-                if (FULL) pre_b[k] += e[k];
-                e[k] *= w[k];
-                s[0] = fmaf(e[k], xh[k], s[0]);
-                if (FULL) s[FULL] += e[k];
-            }
-            P.R.sum(s);
-            const float m1 = s[0] * inv, m0 = layer ? s[FULL] * inv : 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = fmaf(st.w, e[k] - m0 - xh[k] * m1, t[k]);
-        }
-        if (h != nullptr) {
-            parameters(gate, pb, cols, 1.0f, w);
-            parameters(d.post_weight, pb, cols, 1.0f, v);
-            float s[FULL ? 2 : 1] = {};
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (!cols.has(k)) t[k] = 0.0f;
-                post[k] = fmaf(t[k], hh[k], post[k]);
-                if (FULL) post_b[k] += t[k];
-                v[k] *= w[k] * t[k];   // u
-                s[0] = fmaf(v[k], hh[k], s[0]);
-                if (FULL) s[FULL] += v[k];
-                t[k] *= d.residual_scale;
-            }
-            store(static_cast<XT*>(g.grad_x) + r * d.dim, cols, t);
-            P.R.sum(s);
-            const float u1 = s[0] * inv, u0 = layer ? s[FULL] * inv : 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = st.y * (v[k] - u0 - hh[k] * u1);
-            store(static_cast<HT*>(g.grad_h) + r * d.dim, cols, v);
+    // Adds to a sum in shared memory; kinds 4 and 5 are the group's.
+    const auto add_to = [&](int kind, const Cols<VECTOR>& c, const F8& v) {
+        if constexpr (VECTOR) {
+            if (!c.has(0)) return;
+            float4* q = reinterpret_cast<float4*>(place_of(kind, c, 0));
+            float4 a = q[0], b = q[1];
+            a.x += v[0].x; a.y += v[0].y; a.z += v[1].x; a.w += v[1].y;
+            b.x += v[2].x; b.y += v[2].y; b.z += v[3].x; b.w += v[3].y;
+            q[0] = a;
+            q[1] = b;
         } else {
-            store(static_cast<XT*>(g.grad_x) + r * d.dim, cols, t);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (c.has(k)) *place_of(kind, c, k) += value(v, k);
+        }
+    };
+    if (!kRegs) {
+        for (int i = threadIdx.x; i < (GROUPED ? 6 : kKinds) * G.share; i += blockDim.x) shared[i] = 0.0f;
+        __syncthreads();
+    }
+    // With one chunk the parameters and a row's values stay in registers between
+    // its two steps, and where the loads of two rows fit as well, the next row is
+    // loaded ahead.
+    constexpr bool kAhead = I * (sizeof(XT) + sizeof(HT)) <= (FULL ? 4 : 6);
+    F8 kp, kb, kw;
+    if (kRegs) parameters(d.pre_weight, pb, cols, 1.0f, kw);
+    GradRaw<XT, HT, VECTOR> next[I];
+    float4 nst = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const XT *xr = x + r0 * d.x_stride, *gxr = gx + r0 * g.grad_new_stride;
+    const HT *hr = h + r0 * d.h_stride, *gnr = gn + r0 * g.grad_n_stride;
+    const float4* sr = reinterpret_cast<const float4*>(d.stats) + r0;
+    const auto fetch = [&] {   // the next row
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const Cols<VECTOR> c = cols.chunk(i);
+            if (h != nullptr) next[i].h.load(hr, c);
+            next[i].x.load(xr, c);
+            if (gn != nullptr) next[i].gn.load(gnr, c);
+            if (gx != nullptr) next[i].gx.load(gxr, c);
+        }
+        nst = __ldg(sr++);
+        xr += d.x_stride;
+        hr += d.h_stride;
+        gxr += g.grad_new_stride;
+        gnr += g.grad_n_stride;
+    };
+    XT* xo = static_cast<XT*>(g.grad_x) + r0 * d.dim;
+    HT* ho = static_cast<HT*>(g.grad_h) + r0 * d.dim;
+    if (kAhead && r0 < r1) fetch();
+    int64_t turn = r0;   // the row at which another row of the gate begins
+    // The rows of every CTA of a cluster are the same, so all take part in its sums.
+    for (int64_t r = r0; r < r1; ++r, xo += d.dim, ho += d.dim) {
+        if (!kAhead) fetch();
+        GradRaw<XT, HT, VECTOR> raw[I];
+#pragma unroll
+        for (int i = 0; i < I; ++i) raw[i] = next[i];
+        const float4 st = nst;
+        if (kAhead && r + 1 < r1) fetch();
+        const void* gate = d.gate;
+        if (GROUPED && d.gate_rows > 1)
+            gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
+        if (kRegs && r == turn) {
+            fill(kp, 0.0f);
+            if (h != nullptr) post_parameters<FULL>(d, gate, pb, cols, kp, kb);
+            turn = GROUPED ? (r / per + 1) * per : r1;
+        }
+
+        // hh, xh, e and p of a chunk; outside of the row e and p are 0
+        const auto values = [&](int i, const Cols<VECTOR>& c, F8& hh, F8& xh, F8& e, F8& p) {
+            F8 b;
+            raw[i].x.get(xh);
+            if (h != nullptr) {
+                raw[i].h.get(hh);
+                if constexpr (kRegs) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        p[j] = kp[j];
+                        if (FULL) b[j] = kb[j];
+                    }
+                } else {
+                    post_parameters<FULL>(d, gate, pb, c, p, b);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (FULL) hh[j] = add(hh[j], both(-st.x));
+                    hh[j] = mul(hh[j], both(st.y));
+                    if (FULL) xh[j] = fma(both(d.residual_scale), xh[j], b[j]);
+                    else xh[j] = mul(both(d.residual_scale), xh[j]);
+                    xh[j] = fma(p[j], hh[j], xh[j]);
+                }
+            } else {
+                fill(hh, 0.0f);
+                fill(p, 0.0f);
+            }
+            raw[i].gn.get(e);
+            if constexpr (kRegs) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b[j] = kw[j];
+            } else {
+                parameters(d.pre_weight, pb, c, 1.0f, b);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (FULL) xh[j] = add(xh[j], both(-st.z));
+                xh[j] = mul(xh[j], both(st.w));
+                e[j] = mul(e[j], b[j]);
+            }
+        };
+        F8 hh, xh, e, p;
+        float2 s2[FULL ? 10 : 4];
+#pragma unroll
+        for (int j = 0; j < (FULL ? 10 : 4); ++j) s2[j] = both(0.0f);
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            F8 dx;
+            values(i, cols.chunk(i), hh, xh, e, p);
+            raw[i].gx.get(dx);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 q = mul(p[j], hh[j]);
+                s2[0] = fma(e[j], xh[j], s2[0]);
+                s2[1] = fma(dx[j], q, s2[1]);
+                s2[2] = fma(e[j], q, s2[2]);
+                s2[3] = fma(xh[j], q, s2[3]);
+                if constexpr (FULL) {
+                    s2[4] = add(s2[4], e[j]);
+                    s2[5] = add(s2[5], q);
+                    s2[6] = fma(dx[j], p[j], s2[6]);
+                    s2[7] = fma(e[j], p[j], s2[7]);
+                    s2[8] = fma(xh[j], p[j], s2[8]);
+                    s2[9] = add(s2[9], p[j]);
+                }
+            }
+        }
+        float s[1 << kLog] = {};
+#pragma unroll
+        for (int j = 0; j < (FULL ? 10 : 4); ++j) s[j] = s2[j].x + s2[j].y;
+        P.R.template sum<kLog>(s);
+        const float m1 = s[0] * inv;
+        float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(st.w, s[2] - m1 * s[3], s[1]);
+        if constexpr (FULL) {
+            if (layer) {
+                m0 = s[4] * inv;
+                u1 = fmaf(st.w, s[2] - m0 * s[5] - m1 * s[3], s[1]);
+                u0 = fmaf(st.w, s[7] - m0 * s[9] - m1 * s[8], s[6]) * inv;
+            }
+        }
+        u1 *= inv;
+        const float rx = gn != nullptr ? st.w : 0.0f, a = h != nullptr ? d.residual_scale : 1.0f;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const Cols<VECTOR> c = cols.chunk(i);
+            F8 t, dn, o;
+            if (!kRegs) values(i, c, hh, xh, e, p);
+            raw[i].gx.get(t);
+            raw[i].gn.get(dn);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float2 y = fma(xh[j], both(-m1), e[j]);
+                if (FULL) y = add(y, both(-m0));
+                t[j] = fma(both(rx), y, t[j]);
+                if constexpr (kRegs) {
+                    acc[kPre][j] = fma(dn[j], xh[j], acc[kPre][j]);
+                    if (FULL) acc[FULL ? kPreBias : 0][j] = add(acc[FULL ? kPreBias : 0][j], dn[j]);
+                } else {
+                    xh[j] = mul(xh[j], dn[j]);
+                }
+                o[j] = mul(both(a), t[j]);
+            }
+            if constexpr (!kRegs) {
+                add_to(kPre, c, xh);
+                if (FULL) add_to(kPreBias, c, dn);
+            }
+            store(xo, c, o);
+            if (h == nullptr) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = mul(t[j], p[j]);
+                if (FULL) o[j] = add(o[j], both(-u0));
+                o[j] = mul(both(st.y), fma(hh[j], both(-u1), o[j]));
+            }
+            store(ho, c, o);
+            if constexpr (kRegs) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (GROUPED) {
+                        group[0][j] = fma(t[j], hh[j], group[0][j]);
+                        group[1][j] = add(group[1][j], t[j]);
+                    } else {
+                        acc[kPost][j] = fma(t[j], hh[j], acc[kPost][j]);
+                        if (FULL) acc[FULL ? kPostBias : 0][j] = add(acc[FULL ? kPostBias : 0][j], t[j]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) hh[j] = mul(hh[j], t[j]);
+                add_to(GROUPED ? 4 : kPost, c, hh);
+                if (FULL) add_to(GROUPED ? 5 : kPostBias, c, t);
+            }
         }
         if constexpr (GROUPED) {
             if (r + 1 == r1 || (r + 1) % per == 0) {   // the group ends, or this team's part of it
                 const int64_t k0 = r / per, first = k0 * per, last = first + per - 1;
                 const bool whole = first >= r0 && last < r1;
                 float* edge = W.edges + ((P.index * 2 + (first >= r0)) * 2) * d.dim;
-                parameters(gate, pb, cols, 1.0f, w);
-                float w1[8], b1[8];
-                parameters(d.post_weight, pb, cols, 1.0f, w1);
-                parameters(FULL ? d.post_bias : nullptr, pb, cols, 0.0f, b1);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    all[k] = fmaf(w[k], post[k], all[k]);
-                    const float pb_k = FULL ? post_b[FULL ? k : 0] : 0.0f;
-                    if (FULL) all_b[FULL ? k : 0] = fmaf(w[k], pb_k, all_b[FULL ? k : 0]);
-                    if (cols.has(k)) {
-                        if (whole) {
-                            store_any(g.grad_gate, pb, k0 * d.dim + cols.at(k),
-                                      fmaf(w1[k], post[k], b1[k] * pb_k));
+                for (int i = 0; i < I; ++i) {
+                    const Cols<VECTOR> c = cols.chunk(i);
+                    F8 w, w1, b1;
+                    parameters(gate, pb, c, 1.0f, w);
+                    parameters(d.post_weight, pb, c, 1.0f, w1);
+                    parameters(FULL ? d.post_bias : nullptr, pb, c, 0.0f, b1);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (!c.has(k)) continue;
+                        float sum, sum_b;
+                        if constexpr (kRegs) {
+                            sum = value(group[0], k);
+                            sum_b = value(group[GROUPED ? 1 : 0], k);
+                            set(acc[kPost], k, fmaf(value(w, k), sum, value(acc[kPost], k)));
+                            if (FULL)
+                                set(acc[FULL ? kPostBias : 0], k,
+                                    fmaf(value(w, k), sum_b, value(acc[FULL ? kPostBias : 0], k)));
                         } else {
-                            edge[cols.at(k)] = post[k];
-                            edge[d.dim + cols.at(k)] = pb_k;
+                            sum = *place_of(4, c, k);
+                            sum_b = *place_of(5, c, k);
+                            *place_of(kPost, c, k) += value(w, k) * sum;
+                            if (FULL) *place_of(kPostBias, c, k) += value(w, k) * sum_b;
+                            *place_of(4, c, k) = *place_of(5, c, k) = 0.0f;
+                        }
+                        if (whole) {
+                            if (g.grad_gate != nullptr)
+                                store_any(g.grad_gate, pb, k0 * d.dim + c.at(k),
+                                          fmaf(value(w1, k), sum, value(b1, k) * sum_b));
+                        } else {
+                            edge[c.at(k)] = sum;
+                            edge[d.dim + c.at(k)] = sum_b;
                         }
                     }
-                    post[k] = 0.0f;
-                    if (FULL) post_b[FULL ? k : 0] = 0.0f;
+                }
+                if (kRegs) {
+                    fill(group[0], 0.0f);
+                    fill(group[GROUPED && kRegs ? 1 : 0], 0.0f);
                 }
             }
         }
     }
-    if constexpr (GROUPED) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            post[k] = all[k];
-            if (FULL) post_b[FULL ? k : 0] = all_b[FULL ? k : 0];
-        }
-    }
-    // The CTA's sums: its teams add theirs in turn.
-    constexpr int kKinds = FULL ? 4 : 2;
-    const int c0 = P.R.rank * G.share;
     float* out = W.sums + (int64_t)(blockIdx.x / P.R.ctas) * 4 * d.dim;
-    for (int i = 0; i < G.teams; ++i) {
-        if (i > 0) __syncthreads();
-        if (P.team != i) continue;
+    if constexpr (kRegs) {
+        // The CTA's sums: its teams add theirs in turn.
+        for (int i = 0; i < G.teams; ++i) {
+            if (i > 0) __syncthreads();
+            if (P.team != i) continue;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (!cols.has(k)) continue;
-            const float mine[4] = {pre[k], post[k], FULL ? pre_b[FULL ? k : 0] : 0.0f,
-                                   FULL ? post_b[FULL ? k : 0] : 0.0f};
+            for (int k = 0; k < 8; ++k) {
+                if (!cols.has(k)) continue;
 #pragma unroll
-            for (int j = 0; j < kKinds; ++j) {
-                float* s = shared + j * G.share + cols.at(k) - c0;
-                const float v = i > 0 ? *s + mine[j] : mine[j];
-                if (i + 1 < G.teams) *s = v;
-                else out[j * d.dim + cols.at(k)] = v;
+                for (int j = 0; j < kKinds; ++j) {
+                    float* q = place_of(j, cols, k);
+                    const float v = i > 0 ? *q + value(acc[j], k) : value(acc[j], k);
+                    if (i + 1 < G.teams) *q = v;
+                    else out[j * d.dim + cols.at(k)] = v;
+                }
             }
         }
+    } else {
+        __syncthreads();
+        const int mine = max(0, min((int)d.dim - c0, G.share));
+#pragma unroll
+        for (int j = 0; j < kKinds; ++j)
+            for (int i = threadIdx.x; i < mine; i += blockDim.x)
+                out[j * d.dim + c0 + i] = shared[j * G.share + i];
     }
     if (P.R.ctas > 1) cg::this_cluster().sync();
 }
 
+// Waits for copies that ran out.
+static __device__ unsigned int g_norm_timeouts;
+
+// The same for rows on 16-byte boundaries and many of them: a team's rows come
+// through a ring of `stages` in shared memory by bulk copies that one thread
+// issues ahead, so that no registers hold loads and several rows are on their way
+// at any time.  One chunk of columns a thread; wider rows take a cluster.
+template <typename XT, typename HT, bool FULL, bool GROUPED>
+__global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_constant__
+                                                             mdq_residual_norm_grad_desc g,
+                                                             const __grid_constant__ Teams G,
+                                                             const __grid_constant__ Partials W,
+                                                             int stages) {
+    constexpr int kLog = FULL ? 4 : 2, kKinds = FULL ? 4 : 2;
+    __shared__ float slots[2 * kSlots * (1 << kLog)];
+    __shared__ unsigned long long full[kTeam / 32][kMaxStages];
+    extern __shared__ __align__(16) char ring[];   // [team][stage]: h, x, grad_n, grad_new, stats
+    const mdq_residual_norm_desc& d = g.f;
+    Place<true> P(G, (int)d.dim, slots, kSlots << kLog);
+    const Cols<true>& cols = P.cols;
+    const bool layer = FULL && d.kind == MDQ_NORM_LAYER, pb = d.param_dtype == MDQ_BF16;
+    const float inv = 1.0f / (float)d.dim;
+    const int64_t per = d.rows / d.gate_rows;
+    const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
+    const int c0 = P.R.rank * G.share, mine = max(0, cols.end - c0);
+    const bool has_h = d.h != nullptr, has_gn = g.grad_n != nullptr, has_gx = g.grad_new != nullptr;
+
+    const int at_x = G.share * (int)sizeof(HT), at_gn = at_x + G.share * (int)sizeof(XT);
+    const int at_gx = at_gn + G.share * (int)sizeof(HT), at_st = at_gx + G.share * (int)sizeof(XT);
+    const int stage_bytes = at_st + 16;
+    char* stage0 = ring + (size_t)P.team * stages * stage_bytes;
+    // Threads behind the row's end read its last values; their parameters are 0,
+    // and so is what they add.  An absent array's place holds zeros.
+    const int at = min(8 * P.t, mine - 8);
+    for (int k = 0; k < stages; ++k) {
+        char* q = stage0 + k * stage_bytes;
+        const F8 zero = {};
+        if (!has_h) to_shared<HT>(q, at, zero);
+        if (!has_gn) to_shared<HT>(q + at_gn, at, zero);
+        if (!has_gx) to_shared<XT>(q + at_gx, at, zero);
+    }
+    if (P.t == 0)
+        for (int k = 0; k < stages; ++k) bar_init(&full[P.team][k], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (P.R.ctas > 1) cg::this_cluster().sync();
+    else __syncthreads();
+
+    // Copies of the next row into a stage, by the team's first thread.
+    const unsigned long long policy = read_once();
+    int64_t ahead = r0;
+    int to = 0;
+    const auto copy_row = [&] {
+        if (ahead >= r1) return;
+        char* s = stage0 + to * stage_bytes;
+        unsigned long long* bar = &full[P.team][to];
+        const unsigned hb = (unsigned)mine * sizeof(HT), xb = (unsigned)mine * sizeof(XT);
+        const auto part = [&](int place, const void* from, unsigned bytes) {
+            copy_part(bar, s + place, from, bytes, policy);
+        };
+        expect_bytes(bar, (has_h ? hb : 0) + xb + (has_gn ? hb : 0) + (has_gx ? xb : 0) + 16);
+        {
+            if (has_h) part(0, static_cast<const HT*>(d.h) + ahead * d.h_stride + c0, hb);
+            part(at_x, static_cast<const XT*>(d.x) + ahead * d.x_stride + c0, xb);
+            if (has_gn) part(at_gn, static_cast<const HT*>(g.grad_n) + ahead * g.grad_n_stride + c0, hb);
+            if (has_gx) part(at_gx, static_cast<const XT*>(g.grad_new) + ahead * g.grad_new_stride + c0, xb);
+        }
+        part(at_st, d.stats + 4 * ahead, 16);
+        ++ahead;
+        if (++to == stages) to = 0;
+    };
+    if (P.t == 0)
+        for (int k = 0; k < stages - 1; ++k) copy_row();
+
+    F8 acc[kKinds], group[GROUPED ? 2 : 1], kp, kb, kw;
+#pragma unroll
+    for (int j = 0; j < kKinds; ++j) fill(acc[j], 0.0f);
+#pragma unroll
+    for (int j = 0; j < (GROUPED ? 2 : 1); ++j) fill(group[j], 0.0f);
+    parameters(d.pre_weight, pb, cols, 1.0f, kw);
+    XT* xo = static_cast<XT*>(g.grad_x) + r0 * d.dim;
+    HT* ho = static_cast<HT*>(g.grad_h) + r0 * d.dim;
+    const float a = has_h ? d.residual_scale : 1.0f;
+    int64_t turn = r0;   // the row at which another row of the gate begins
+    int stage = 0;
+    unsigned phase = 0;
+    bool lost = false;
+    // The rows of every CTA of a cluster are the same, so all take part in its sums.
+    for (int64_t r = r0; r < r1; ++r, xo += d.dim, ho += d.dim) {
+        const void* gate = d.gate;
+        if (GROUPED) gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
+        if (r == turn) {
+            fill(kp, 0.0f);
+            fill(kb, 0.0f);
+            if (has_h) post_parameters<FULL>(d, gate, pb, cols, kp, kb);
+            turn = GROUPED ? (r / per + 1) * per : r1;
+        }
+        if (!lost && !bar_wait(&full[P.team][stage], phase)) {
+            lost = true;   // the results become NaN
+            if (P.t == 0) atomicAdd(&g_norm_timeouts, 1u);
+        }
+        const char* s0 = stage0 + stage * stage_bytes;
+        const float4 st = lost ? make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F)
+                               : *reinterpret_cast<const float4*>(s0 + at_st);
+        F8 hh, xh, dx, dn;
+        from_shared<XT>(s0 + at_x, at, xh);
+        from_shared<HT>(s0 + at_gn, at, dn);
+        from_shared<XT>(s0 + at_gx, at, dx);
+        from_shared<HT>(s0, at, hh);
+        float2 s2[FULL ? 10 : 4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (FULL) hh[j] = add(hh[j], both(-st.x));
+            hh[j] = mul(hh[j], both(st.y));
+            const float2 q = mul(kp[j], hh[j]), e = mul(dn[j], kw[j]);
+            if (FULL) xh[j] = fma(both(a), xh[j], add(add(kb[j], both(-st.z)), q));
+            else xh[j] = fma(both(a), xh[j], q);
+            xh[j] = mul(xh[j], both(st.w));
+            const auto take = [&](int i, float2 x, float2 y) { s2[i] = j == 0 ? mul(x, y) : fma(x, y, s2[i]); };
+            take(0, e, xh[j]);
+            take(1, dx[j], q);
+            take(2, e, q);
+            take(3, xh[j], q);
+            if constexpr (FULL) {
+                s2[4] = j == 0 ? e : add(s2[4], e);
+                s2[5] = j == 0 ? q : add(s2[5], q);
+                take(6, dx[j], kp[j]);
+                take(7, e, kp[j]);
+                take(8, xh[j], kp[j]);
+                s2[9] = j == 0 ? kp[j] : add(s2[9], kp[j]);
+            }
+        }
+        float s[1 << kLog] = {};
+#pragma unroll
+        for (int j = 0; j < (FULL ? 10 : 4); ++j) s[j] = s2[j].x + s2[j].y;
+        P.R.template sum<kLog>(s);
+        // Every thread is past the row before (a warp alone: in step): its stage is free.
+        if (G.threads == 32) __syncwarp();
+        if (P.t == 0 && !lost) copy_row();
+        const float m1 = s[0] * inv;
+        float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(st.w, s[2] - m1 * s[3], s[1]);
+        if constexpr (FULL) {
+            if (layer) {
+                m0 = s[4] * inv;
+                u1 = fmaf(st.w, s[2] - m0 * s[5] - m1 * s[3], s[1]);
+                u0 = fmaf(st.w, s[7] - m0 * s[9] - m1 * s[8], s[6]) * inv;
+            }
+        }
+        u1 *= inv;
+        const float rx = has_gn ? st.w : 0.0f;
+        F8 o;
+        if (FULL) {   // read again: the registers were the sums'
+            from_shared<HT>(s0 + at_gn, at, dn);
+            from_shared<XT>(s0 + at_gx, at, dx);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 y = fma(dn[j], kw[j], both(-m0));
+            y = fma(xh[j], both(-m1), y);
+            dx[j] = fma(both(rx), y, dx[j]);   // the whole gradient of x_new
+            acc[kPre][j] = fma(dn[j], xh[j], acc[kPre][j]);
+            if (FULL) acc[FULL ? kPreBias : 0][j] = add(acc[FULL ? kPreBias : 0][j], dn[j]);
+            o[j] = mul(both(a), dx[j]);
+        }
+        store(xo, cols, o);
+        if (has_h) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = mul(dx[j], kp[j]);
+                if (FULL) o[j] = add(o[j], both(-u0));
+                o[j] = mul(both(st.y), fma(hh[j], both(-u1), o[j]));
+                if constexpr (GROUPED) {
+                    group[0][j] = fma(dx[j], hh[j], group[0][j]);
+                    group[GROUPED ? 1 : 0][j] = add(group[GROUPED ? 1 : 0][j], dx[j]);
+                } else {
+                    acc[kPost][j] = fma(dx[j], hh[j], acc[kPost][j]);
+                    if (FULL) acc[FULL ? kPostBias : 0][j] = add(acc[FULL ? kPostBias : 0][j], dx[j]);
+                }
+            }
+            store(ho, cols, o);
+        }
+        if constexpr (GROUPED) {
+            if (r + 1 == r1 || r + 1 == turn) {   // the group ends, or this team's part of it
+                const int64_t k0 = r / per, first = k0 * per, last = first + per - 1;
+                float* edge = nullptr;
+                if (first < r0 || last >= r1) edge = W.edges + ((P.index * 2 + (first >= r0)) * 2) * d.dim;
+                end_group<true, FULL>(g, gate, pb, cols, k0, edge, group, acc);
+            }
+        }
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    if (lost && P.t == 0)   // copies still on their way end before the CTA does
+        for (int64_t k = ahead - min(ahead - r0, (int64_t)stages); k < ahead; ++k)
+            bar_wait(&full[P.team][(k - r0) % stages], (unsigned)((k - r0) / stages) & 1);
+    __syncthreads();
+    end_sums<true, kKinds>(P, G, W, (int)d.dim, reinterpret_cast<float*>(ring), acc);
+    if (P.R.ctas > 1) cg::this_cluster().sync();
+}
+
+template <typename XT, typename HT, bool VECTOR>
+cudaError_t run_forward(const mdq_residual_norm_desc& d, const Teams& G, int chunks, int grid,
+                        int cluster, bool full, cudaStream_t stream) {
+    typedef void (*Kernel)(const mdq_residual_norm_desc, const Teams);
+    const Kernel k = chunks == 1   ? (full ? (Kernel)norm_rows<XT, HT, VECTOR, 1, true>
+                                           : (Kernel)norm_rows<XT, HT, VECTOR, 1, false>)
+                     : chunks == 2 ? (full ? (Kernel)norm_rows<XT, HT, VECTOR, 2, true>
+                                           : (Kernel)norm_rows<XT, HT, VECTOR, 2, false>)
+                                   : (full ? (Kernel)norm_rows<XT, HT, VECTOR, 4, true>
+                                           : (Kernel)norm_rows<XT, HT, VECTOR, 4, false>);
+    return launch(k, dim3(grid), G.threads * G.teams, 0, stream, cluster, false, d, G);
+}
+
 template <typename XT, typename HT>
-cudaError_t run_forward(const mdq_residual_norm_desc& d, const Teams& G, int grid, int cluster,
-                        bool vector, cudaStream_t stream) {
-    const int threads = G.threads * G.teams;
-    return vector ? launch(norm_rows<XT, HT, true>, dim3(grid), threads, 0, stream, cluster, false, d, G)
-                  : launch(norm_rows<XT, HT, false>, dim3(grid), threads, 0, stream, cluster, false, d, G);
+cudaError_t run_stream(const mdq_residual_norm_grad_desc& g, const Teams& G, const Partials& W,
+                       int stages, size_t smem, int grid, int cluster, bool full, bool grouped,
+                       cudaStream_t stream) {
+    typedef void (*Kernel)(const mdq_residual_norm_grad_desc, const Teams, const Partials, int);
+    const Kernel k = full ? (grouped ? (Kernel)norm_grad_stream<XT, HT, true, true>
+                                     : (Kernel)norm_grad_stream<XT, HT, true, false>)
+                          : (grouped ? (Kernel)norm_grad_stream<XT, HT, false, true>
+                                     : (Kernel)norm_grad_stream<XT, HT, false, false>);
+    return launch<209 * 1024>(k, dim3(grid), G.threads * G.teams, smem, stream, cluster, false, g, G, W,
+                              stages);
 }
 
 template <typename XT, typename HT, bool VECTOR>
 cudaError_t run_backward(const mdq_residual_norm_grad_desc& g, const Teams& G, const Partials& W,
-                         int grid, int cluster, bool full, bool grouped, cudaStream_t stream) {
-    const int threads = G.threads * G.teams;
-    const size_t smem = G.teams > 1 ? sizeof(float) * (full ? 4 : 2) * G.share : 0;
+                         int chunks, int grid, int cluster, bool full, bool grouped,
+                         cudaStream_t stream) {
+    const int kinds = chunks > 1 ? (grouped ? 6 : full ? 4 : 2) : G.teams > 1 ? (full ? 4 : 2) : 0;
     typedef void (*Kernel)(const mdq_residual_norm_grad_desc, const Teams, const Partials);
-    const Kernel k = full ? (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, true, true>
-                                     : (Kernel)norm_grad_rows<XT, HT, VECTOR, true, false>)
-                          : (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, false, true>
-                                     : (Kernel)norm_grad_rows<XT, HT, VECTOR, false, false>);
-    return launch(k, dim3(grid), threads, smem, stream, cluster, false, g, G, W);
+    const Kernel k =
+        chunks == 1 ? (full ? (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, true, true>
+                                       : (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, true, false>)
+                            : (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, false, true>
+                                       : (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, false, false>))
+        : chunks == 2 ? (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, true, true>
+                         : full  ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, true, false>
+                                 : (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, false, false>)
+                      : (Kernel)norm_grad_rows<XT, HT, VECTOR, 4, false, false>;
+    return launch<210 * 1024>(k, dim3(grid), G.threads * G.teams, sizeof(float) * kinds * G.share,
+                              stream, cluster, false, g, G, W);
 }
 
 #define MDQ_NORM_TYPES(DECL)                                                                       \
     DECL(float, float, ff) DECL(float, __nv_bfloat16, fb) DECL(__nv_bfloat16, __nv_bfloat16, bb)   \
         DECL(__nv_bfloat16, float, bf)
 #define MDQ_NORM_DECLARE(XT, HT, S)                                                                \
-    cudaError_t forward_##S(const mdq_residual_norm_desc&, const Teams&, int, int, bool,           \
-                            cudaStream_t);                                                         \
+    cudaError_t forward_##S(const mdq_residual_norm_desc&, const Teams&, int, int, int, bool,      \
+                            bool, cudaStream_t);                                                   \
     cudaError_t backward_##S(const mdq_residual_norm_grad_desc&, const Teams&, const Partials&,    \
-                             int, int, bool, bool, bool, cudaStream_t);
+                             int, int, int, bool, bool, bool, cudaStream_t);                       \
+    cudaError_t stream_##S(const mdq_residual_norm_grad_desc&, const Teams&, const Partials&, int, \
+                           size_t, int, int, bool, bool, cudaStream_t);
 MDQ_NORM_TYPES(MDQ_NORM_DECLARE)
 
 // The kernels of one pair of types (x, h), in a file of its own.
 #define MDQ_NORM_INSTANTIATE(XT, HT, S)                                                            \
     namespace mdq_norm {                                                                           \
-    cudaError_t forward_##S(const mdq_residual_norm_desc& d, const Teams& G, int grid,             \
-                            int cluster, bool vector, cudaStream_t stream) {                       \
-        return run_forward<XT, HT>(d, G, grid, cluster, vector, stream);                           \
+    cudaError_t forward_##S(const mdq_residual_norm_desc& d, const Teams& G, int chunks, int grid, \
+                            int cluster, bool vector, bool full, cudaStream_t stream) {            \
+        return vector ? run_forward<XT, HT, true>(d, G, chunks, grid, cluster, full, stream)       \
+                      : run_forward<XT, HT, false>(d, G, chunks, grid, cluster, full, stream);     \
     }                                                                                              \
     cudaError_t backward_##S(const mdq_residual_norm_grad_desc& g, const Teams& G,                 \
-                             const Partials& W, int grid, int cluster, bool vector, bool full,     \
-                             bool grouped, cudaStream_t stream) {                                  \
-        return vector                                                                              \
-                   ? run_backward<XT, HT, true>(g, G, W, grid, cluster, full, grouped, stream)     \
-                   : run_backward<XT, HT, false>(g, G, W, grid, cluster, full, grouped, stream);   \
+                             const Partials& W, int chunks, int grid, int cluster, bool vector,    \
+                             bool full, bool grouped, cudaStream_t stream) {                       \
+        return vector ? run_backward<XT, HT, true>(g, G, W, chunks, grid, cluster, full, grouped,  \
+                                                   stream)                                         \
+                      : run_backward<XT, HT, false>(g, G, W, chunks, grid, cluster, full, grouped, \
+                                                    stream);                                       \
+    }                                                                                              \
+    cudaError_t stream_##S(const mdq_residual_norm_grad_desc& g, const Teams& G, const Partials& W,\
+                           int stages, size_t smem, int grid, int cluster, bool full,              \
+                           bool grouped, cudaStream_t stream) {                                    \
+        return run_stream<XT, HT>(g, G, W, stages, smem, grid, cluster, full, grouped, stream);    \
     }                                                                                              \
     }
 

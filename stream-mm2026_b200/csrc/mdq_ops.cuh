@@ -48,6 +48,56 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// ---- bulk copies into shared memory
+
+__device__ __forceinline__ unsigned smem_at(const void* p) {
+    return (unsigned)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void bar_init(void* bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_at(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(void* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory");
+}
+
+// Whether the barrier's phase ended.  Phases last microseconds; the limit
+// (hundreds of milliseconds) only keeps a lost copy from hanging the GPU.
+__device__ __forceinline__ bool bar_wait(void* bar, unsigned parity) {
+    for (int i = 0; i < 1 << 22; ++i) {
+        unsigned done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(smem_at(bar)), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ unsigned long long read_once() {   // evict-first in L2
+    unsigned long long policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+// Arrives at the barrier, which `bytes` of copies (may be 0) end on as well.
+__device__ __forceinline__ void expect_bytes(void* bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_part(void* bar, void* to, const void* from, unsigned bytes,
+                                          unsigned long long policy) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1], %2, [%3], %4;" ::"r"(smem_at(to)),
+        "l"(from), "r"(bytes), "r"(smem_at(bar)), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ void copy_in(void* bar, void* to, const void* from, unsigned bytes,
+                                        unsigned long long policy) {
+    expect_bytes(bar, bytes);
+    if (bytes > 0) copy_part(bar, to, from, bytes, policy);
+}
+
 inline bool float_type(int32_t t) { return t == MDQ_F32 || t == MDQ_BF16; }
 inline bool id_type(int32_t t) { return t == MDQ_I32 || t == MDQ_I64; }
 
@@ -98,20 +148,20 @@ inline bool rows16(const void* p, int64_t stride, int32_t type) {
 }
 inline int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
 
-// Dynamic shared memory a kernel may ask for (227 KB less its static arrays,
-// which stay below 4 KB).
+// Dynamic shared memory a kernel may ask for: 227 KB less its static arrays,
+// which stay below 4 KB (launch<MOST> where they do not).
 constexpr int kMaxShared = 223 * 1024;
 
 // One launch.  With `dependent` the grid may be set up while the previous
 // kernel of the stream still runs; it calls wait_previous() before it reads
 // what that kernel wrote (programmatic dependent launch).
-template <typename... P, typename... A>
+template <int MOST = kMaxShared, typename... P, typename... A>
 inline cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
                           cudaStream_t stream, int cluster, bool dependent, A... args) {
     if (smem > 48 * 1024) {   // always the same limit: calls of other threads may set it as well
         const cudaError_t e = cudaFuncSetAttribute(
             reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-            kMaxShared);
+            MOST);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchAttribute at[2];
