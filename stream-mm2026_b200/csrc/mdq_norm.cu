@@ -195,36 +195,63 @@ __global__ void __launch_bounds__(kThreads) norm_grad_wide_columns(const __grid_
 // ------------------------------------------------------------- sums over CTAs
 
 // Adds the CTAs' sums of 32 columns, a warp every 16th CTA, and the warps' sums
-// in order; forms the parameters' gradients from them.  blockIdx.y: pre or post
-// norm.
+// in order; forms the parameters' gradients from them.  blockIdx.y: the norm
+// before, the norm behind, and then rows of the gate whose group no team had
+// whole, from the teams' sums of it.
 __global__ void __launch_bounds__(512) norm_grad_sum(const __grid_constant__
                                                      mdq_residual_norm_grad_desc g,
                                                      const __grid_constant__ Partials W, int blocks,
-                                                     int full, int grouped) {
+                                                     int run, int full, int grouped) {
     __shared__ float red[2][16][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t dim = g.f.dim, c = (int64_t)blockIdx.x * 32 + lane;
-    const int kind = blockIdx.y;   // kPre or kPost; its bias is two further
-    wait_previous();
-    float s = 0.0f, b = 0.0f;
-    if (c < dim) {
-#pragma unroll 4
-        for (int i = warp; i < blocks; i += 16) {
-            s += W.sums[((int64_t)i * 4 + kind) * dim + c];
-            if (full) b += W.sums[((int64_t)i * 4 + kind + 2) * dim + c];
-        }
-    }
-    red[0][warp][lane] = s;
-    red[1][warp][lane] = b;
-    __syncthreads();
-    if (warp != 0 || c >= dim) return;
-    s = b = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        s += red[0][k][lane];
-        b += red[1][k][lane];
-    }
     const bool pb = g.f.param_dtype == MDQ_BF16;
+    // Sums of `count` pairs `step` floats apart from p on, the second of a pair at `other`.
+    const auto total = [&](const float* p, int64_t count, int64_t step, int64_t other, float& s, float& b) {
+        s = b = 0.0f;
+        if (c < dim) {
+#pragma unroll 5
+            for (int64_t i = warp; i < count; i += 16) {
+                s += p[i * step + c];
+                if (full) b += p[i * step + other + c];
+            }
+        }
+        __syncthreads();
+        red[0][warp][lane] = s;
+        red[1][warp][lane] = b;
+        __syncthreads();
+        s = b = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            s += red[0][k][lane];
+            b += red[1][k][lane];
+        }
+    };
+    wait_previous();
+    float s, b;
+    const bool post = c < dim && g.f.h != nullptr && warp == 0 && blockIdx.y > 0;
+    const float w = post ? load_any(g.f.post_weight, pb, c) : 0.0f;
+    const float bias = post && g.f.post_bias != nullptr ? load_any(g.f.post_bias, pb, c) : 0.0f;
+    if (blockIdx.y >= 2) {
+        const int64_t per = g.f.rows / g.f.gate_rows;
+        for (int64_t k = blockIdx.y - 2; k < g.f.gate_rows; k += gridDim.y - 2) {
+            const int64_t first = k * per / run, last = ((k + 1) * per - 1) / run;   // teams
+            if (first == last) continue;
+            // The group began in the first of these teams, and before the others:
+            // the first's second place, then the others' first.
+            total(W.edges + (first * 2 + 2) * 2 * dim, last - first, 4 * dim, dim, s, b);
+            if (post) {
+                const float* edge = W.edges + (first * 2 + 1) * 2 * dim;
+                s += edge[c];
+                if (full) b += edge[dim + c];
+                store_any(g.grad_gate, pb, k * dim + c, fmaf(w, s, bias * b));
+            }
+        }
+        return;
+    }
+    const int kind = blockIdx.y;   // kPre or kPost; its bias is two further
+    total(W.sums + kind * dim, blocks, 4 * dim, 2 * dim, s, b);
+    if (warp != 0 || c >= dim) return;
     if (kind == kPre) {
         if (g.grad_pre_weight != nullptr) store_any(g.grad_pre_weight, pb, c, s);
         if (g.grad_pre_bias != nullptr) store_any(g.grad_pre_bias, pb, c, b);
@@ -235,39 +262,10 @@ __global__ void __launch_bounds__(512) norm_grad_sum(const __grid_constant__
     float gate = 1.0f;
     if (!grouped && g.f.gate != nullptr) {
         gate = load_any(g.f.gate, pb, c);
-        const float w = load_any(g.f.post_weight, pb, c);
-        const float bias = g.f.post_bias == nullptr ? 0.0f : load_any(g.f.post_bias, pb, c);
         if (g.grad_gate != nullptr) store_any(g.grad_gate, pb, c, fmaf(w, s, bias * b));
     }
     if (g.grad_post_weight != nullptr) store_any(g.grad_post_weight, pb, c, gate * s);
     if (g.grad_post_bias != nullptr) store_any(g.grad_post_bias, pb, c, gate * b);
-}
-
-// Rows of the gate whose group no team had whole: the teams' sums in order.
-__global__ void __launch_bounds__(256) norm_grad_gate(const __grid_constant__
-                                                      mdq_residual_norm_grad_desc g,
-                                                      const __grid_constant__ Partials W, int run,
-                                                      int full) {
-    const int64_t dim = g.f.dim, per = g.f.rows / g.f.gate_rows;
-    const bool pb = g.f.param_dtype == MDQ_BF16;
-    wait_previous();
-    for (int64_t k = blockIdx.y; k < g.f.gate_rows; k += gridDim.y) {
-        const int64_t first = k * per / run, last = ((k + 1) * per - 1) / run;   // teams
-        if (first == last) continue;
-        for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < dim; c += (int64_t)gridDim.x * 256) {
-            float s = 0.0f, b = 0.0f;
-#pragma unroll 4
-            for (int64_t i = first; i <= last; ++i) {
-                // The group began in the first of these teams and before the others.
-                const float* edge = W.edges + ((i * 2 + (i == first)) * 2) * dim;
-                s += edge[c];
-                if (full) b += edge[dim + c];
-            }
-            const float w = load_any(g.f.post_weight, pb, c);
-            const float bias = g.f.post_bias == nullptr ? 0.0f : load_any(g.f.post_bias, pb, c);
-            store_any(g.grad_gate, pb, k * dim + c, fmaf(w, s, bias * b));
-        }
-    }
 }
 
 // ------------------------------------------------------------------ planning
@@ -283,6 +281,29 @@ bool plan_columns(int64_t dim, int chunks, int* cluster, Teams* G) {
     while (*cluster < kMaxCluster && dim > *cluster * most) *cluster *= 2;
     if (dim > *cluster * most) return false;
     G->share = (int)(ceil_div(ceil_div(dim, *cluster), kCols) * kCols);
+    return true;
+}
+
+// Bytes of a stage whose arrays take `row_bytes` a column.
+int64_t stage_of(int64_t row_bytes, int arrays, bool vec, const Teams& G, int chunks) {
+    return vec ? row_bytes * G.share : row_bytes * G.threads * kCols * chunks + 48 * arrays;
+}
+// Teams of a CTA: as many as rows for all SMs need, 512 threads at most, and so
+// many stages for each that two rows are on their way, in 200 KB.
+bool plan_ring(int64_t rows, int64_t stage, bool one, Teams* G, int* stages, size_t* smem) {
+    const int64_t room = 200 * 1024;
+    int64_t teams = one ? 1 : kTeam / G->threads;
+    const int64_t need = ceil_div(rows, 148);
+    if (teams > need) teams = need < 1 ? 1 : need;
+    while (teams > 1 && 3 * stage * teams > room) --teams;
+    int64_t n = room / (stage * teams);
+    if (n < 2) return false;
+    const int64_t run = ceil_div(rows, 148 * teams);   // more would not be used
+    if (n > run + 1) n = run + 1 < 2 ? 2 : run + 1;
+    if (n > kMaxStages) n = kMaxStages;
+    G->teams = (int)teams;
+    *stages = (int)n;
+    *smem = (size_t)(n * stage * teams);
     return true;
 }
 
@@ -313,14 +334,11 @@ struct GradPlan {
     int64_t blocks;    // clusters, each with a row of sums
     int64_t bytes;
 };
-// Rows, sums and bytes once columns are given to threads.
+// Rows, sums and bytes once teams are known: one CTA an SM, as their registers go.
 void plan_rows(int64_t rows, int64_t dim, int64_t gate_rows, GradPlan* p) {
     Teams& G = p->G;
-    // One CTA an SM (its registers end there), fewer where few rows would give
-    // teams less than four, so that the sums over CTAs stay short.
     const int64_t most = 148 / p->cluster;
-    int64_t teams = ceil_div(rows, 4);
-    p->blocks = ceil_div(teams, G.teams);
+    p->blocks = ceil_div(rows, G.teams);
     if (p->blocks > most) p->blocks = most;
     if (p->blocks < 1) p->blocks = 1;
     G.run = (int)ceil_div(rows, p->blocks * G.teams);
@@ -335,29 +353,26 @@ bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, bool full, GradPlan
     p->smem = 0;
     if (!plan_columns(dim, wide ? 4 : 2, &p->cluster, &p->G)) return false;
     Teams& G = p->G;
-    p->chunks = 1;
+    p->chunks = 2;
     while (threads_for(G.share, p->chunks) > kTeam) p->chunks *= 2;
     G.threads = threads_for(G.share, p->chunks);
-    G.teams = p->cluster > 1 || p->chunks > 1 ? 1 : kTeam / G.threads;
+    G.teams = 1;
     plan_rows(rows, dim, gate_rows, p);
     return true;
 }
-// The streaming kernel: two rows ahead at least, in 200 KB.
-bool plan_stream(int64_t rows, int64_t dim, int64_t gate_rows, int64_t row_bytes, bool full, GradPlan* p) {
+// With rows in a ring.  Above 8192 columns the steps between more than two CTAs
+// take longer than the other kernel's rows (503 against 382 us for 4096 rows of
+// 16384).
+bool plan_stream(int64_t rows, int64_t dim, int64_t gate_rows, int64_t row_bytes, bool vec, bool full,
+                 GradPlan* p) {
     p->chunks = 1;
-    // Above 8192 columns the steps between more than two CTAs take longer than the
-    // other kernel's rows (503 against 382 us for 4096 rows of 16384).
     if (!plan_columns(dim, 1, &p->cluster, &p->G) || p->cluster > 2) return false;
     Teams& G = p->G;
     G.threads = threads_for(G.share, 1);
-    G.teams = p->cluster > 1 ? 1 : kTeam / G.threads;
-    const int64_t stage = row_bytes * G.share + 16, room = 200 * 1024;
-    while (G.teams > 1 && 3 * stage * G.teams > room) --G.teams;
-    int64_t stages = room / (stage * G.teams);
-    if (stages < 2) return false;
-    p->stages = stages < kMaxStages ? (int)stages : kMaxStages;
-    const int64_t sums = G.teams > 1 ? (full ? 4 : 2) * G.share * (int64_t)sizeof(float) : 0;
-    p->smem = (size_t)(p->stages * stage * G.teams > sums ? p->stages * stage * G.teams : sums);
+    const int64_t stage = stage_of(row_bytes, 4, vec, G, 1) + 16;
+    if (!plan_ring(rows, stage, p->cluster > 1, &G, &p->stages, &p->smem)) return false;
+    const size_t sums = G.teams > 1 ? (full ? 4 : 2) * G.share * sizeof(float) : 0;
+    if (p->smem < sums) p->smem = sums;
     plan_rows(rows, dim, gate_rows, p);
     return true;
 }
@@ -431,12 +446,14 @@ mdq_status mdq_residual_norm_grad_workspace_bytes(int64_t rows, int64_t dim, int
     // Enough for either kind of norm and all types.
     *bytes = rows * 2 * (int64_t)sizeof(float);
     for (int full = 0; full < 2; ++full)
-        for (int row_bytes = 0; row_bytes <= 16; row_bytes += row_bytes < 8 ? 8 : 4) {
-            GradPlan p;
-            const bool ok = row_bytes == 0 ? plan_grad(rows, dim, gate_rows, full, &p)
-                                           : plan_stream(rows, dim, gate_rows, row_bytes, full, &p);
-            if (ok && p.bytes > *bytes) *bytes = p.bytes;
-        }
+        for (int vec = 0; vec < 2; ++vec)
+            for (int row_bytes = 0; row_bytes <= 16; row_bytes += row_bytes < 8 ? 8 : 4) {
+                GradPlan p;
+                const bool ok = row_bytes == 0
+                                    ? plan_grad(rows, dim, gate_rows, full, &p)
+                                    : plan_stream(rows, dim, gate_rows, row_bytes, vec, full, &p);
+                if (ok && p.bytes > *bytes) *bytes = p.bytes;
+            }
     return MDQ_OK;
 }
 
@@ -462,38 +479,34 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: workspace or stats misaligned");
     const bool grouped = g->f.gate_rows > 1;
     const bool full = g->f.kind == MDQ_NORM_LAYER || g->f.post_bias != nullptr || g->f.pre_bias != nullptr;
+    const bool vec = vector_rows(g->f) && aligned16(g->grad_x) && aligned16(g->grad_h) &&
+                     (g->grad_new == nullptr || rows16(g->grad_new, g->grad_new_stride, g->f.x_dtype)) &&
+                     (g->grad_n == nullptr || rows16(g->grad_n, g->grad_n_stride, g->f.h_dtype));
+    const int row_bytes = 2 * (int)(type_size(g->f.x_dtype) + type_size(g->f.h_dtype));
     GradPlan p;
-    if (!plan_grad(g->f.rows, g->f.dim, g->f.gate_rows, full, &p)) {
+    if (!plan_stream(g->f.rows, g->f.dim, g->f.gate_rows, row_bytes, vec, full, &p) &&
+        !plan_grad(g->f.rows, g->f.dim, g->f.gate_rows, full, &p)) {
         float* means = static_cast<float*>(g->workspace);
         if (g->f.rows > 0)
             norm_grad_wide<<<(unsigned)g->f.rows, kThreads, 0, stream>>>(*g, means);
         norm_grad_wide_columns<<<(unsigned)ceil_div(g->f.dim, kThreads), kThreads, 0, stream>>>(*g, means);
         return launch_status("residual norm grad");
     }
-    const bool vec = vector_rows(g->f) && aligned16(g->grad_x) && aligned16(g->grad_h) &&
-                     (g->grad_new == nullptr || rows16(g->grad_new, g->grad_new_stride, g->f.x_dtype)) &&
-                     (g->grad_n == nullptr || rows16(g->grad_n, g->grad_n_stride, g->f.h_dtype));
-    const int row_bytes = 2 * (int)(type_size(g->f.x_dtype) + type_size(g->f.h_dtype));
-    GradPlan q;
-    if (vec && plan_stream(g->f.rows, g->f.dim, g->f.gate_rows, row_bytes, full, &q)) p = q;
     Partials W;
     W.sums = static_cast<float*>(g->workspace);
     W.edges = W.sums + p.blocks * 4 * g->f.dim;
     const int grid = (int)p.blocks * p.cluster;
     st = status_of(p.stages > 0 ? MDQ_NORM_PICK(stream, g->f.x_dtype, g->f.h_dtype)(
-                                      *g, p.G, W, p.stages, p.smem, grid, p.cluster, full, grouped, stream)
+                                      *g, p.G, W, p.stages, p.smem, grid, p.cluster, vec, full, grouped, stream)
                                 : MDQ_NORM_PICK(backward, g->f.x_dtype, g->f.h_dtype)(
                                       *g, p.G, W, p.chunks, grid, p.cluster, vec, full, grouped, stream),
                    "residual norm grad");
     if (st != MDQ_OK) return st;
-    const dim3 columns((unsigned)ceil_div(g->f.dim, 32), g->f.h != nullptr ? 2 : 1);
-    cudaError_t e = launch(norm_grad_sum, columns, 512, 0, stream, 1, true, *g, W, (int)p.blocks, (int)full,
-                           (int)grouped);
-    if (e == cudaSuccess && grouped && g->grad_gate != nullptr) {
-        const int64_t groups = g->f.gate_rows < 256 ? g->f.gate_rows : 256;
-        e = launch(norm_grad_gate, dim3((unsigned)ceil_div(g->f.dim, 256), (unsigned)groups), 256, 0,
-                   stream, 1, false, *g, W, p.G.run, (int)full);
-    }
+    const bool gates = grouped && g->grad_gate != nullptr;
+    const int64_t groups = !gates ? 0 : g->f.gate_rows < 256 ? g->f.gate_rows : 256;
+    const dim3 columns((unsigned)ceil_div(g->f.dim, 32), g->f.h != nullptr ? (unsigned)(2 + groups) : 1);
+    const cudaError_t e = launch(norm_grad_sum, columns, 512, 0, stream, 1, true, *g, W, (int)p.blocks,
+                                 p.G.run, (int)full, (int)grouped);
     return status_of(e, "residual norm grad");
 }
 

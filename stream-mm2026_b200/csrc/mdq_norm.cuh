@@ -129,6 +129,18 @@ __device__ __forceinline__ void store(T* row, const Cols<VECTOR>& c, const F8& v
     }
 }
 
+// Zeros outside of the row, whatever was read there.
+template <bool VECTOR>
+__device__ __forceinline__ void within_row(F8& v, const Cols<VECTOR>& c) {
+    if constexpr (VECTOR) {
+        if (!c.has(0)) fill(v, 0.0f);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (!c.has(k)) set(v, k, 0.0f);
+    }
+}
+
 // Parameters of a chunk: `none` without an array, 0 outside of the row.
 template <bool VECTOR>
 __device__ __forceinline__ void parameters(const void* p, bool bf16, const Cols<VECTOR>& c, float none,
@@ -300,8 +312,9 @@ __device__ __forceinline__ float2 statistics(Reducer& R, const Cols<VECTOR>& col
 }
 
 // I chunks of 8 columns a thread.  With one or two, the parameters stay in
-// registers over a team's rows and the next row is loaded ahead; with four (rows
-// above 8192 columns) neither fits, and a row is long enough to fill the time.
+// registers over a team's rows and the next row is loaded ahead (not where twice
+// as many parameters take the registers); with four (rows above 8192 columns)
+// neither fits, and a row is long enough to fill the time.
 // FULL: layer norm or biases.
 template <typename XT, typename HT, bool VECTOR, int I, bool FULL>
 __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ mdq_residual_norm_desc d,
@@ -316,7 +329,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
     const HT* h = static_cast<const HT*>(d.h);
     const int64_t per = d.rows / d.gate_rows;
     const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
-    constexpr bool kKeep = I <= 2;
+    constexpr bool kKeep = I <= 2, kAhead = kKeep && !(FULL && I == 2);
     F8 kp[kKeep ? I : 1], kb[kKeep && FULL ? I : 1], kw[kKeep ? I : 1], kc[kKeep && FULL ? I : 1];
     if constexpr (kKeep) {
 #pragma unroll
@@ -340,7 +353,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
     };
     XT* xo = static_cast<XT*>(d.x_new) + r0 * d.dim;
     HT* no = static_cast<HT*>(d.n) + r0 * d.dim;
-    if (kKeep && r0 < r1) fetch();
+    if (kAhead && r0 < r1) fetch();
     int64_t turn = r0;   // the row at which another row of the gate begins
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, no += d.dim) {
         const void* gate = d.gate;
@@ -357,13 +370,13 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
         F8 v[I];
         Raw<XT, VECTOR> rx[I];
         float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (!kKeep) fetch();
+        if (!kAhead) fetch();
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             rx[i] = nx[i];
             nh[i].get(v[i]);
         }
-        if (kKeep && r + 1 < r1) fetch();
+        if (kAhead && r + 1 < r1) fetch();
         if (h != nullptr) {
             const float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
             st.x = s.x;
@@ -498,27 +511,76 @@ __device__ __forceinline__ void end_sums(const Place<VECTOR>& P, const Teams& G,
     }
 }
 
-// Eight values of a row in shared memory.
-template <typename T>
-__device__ __forceinline__ void from_shared(const char* row, int at, F8& v) {
-    const T* p = reinterpret_cast<const T*>(row) + at;
-    if constexpr (sizeof(T) == 2) {
-        unpack(*reinterpret_cast<const uint4*>(p), v);
+// ---------------------------------------------------------- rows in a ring
+
+constexpr int kMaxStages = 6;
+
+// Waits for copies that ran out.
+static __device__ unsigned int g_norm_timeouts;
+
+// A chunk's eight values in shared memory, the row's first at `row`.
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void from_shared(const T* row, int at, int step, F8& v) {
+    if constexpr (!VECTOR) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) set(v, k, to_f(row[at + k * step]));
+    } else if constexpr (sizeof(T) == 2) {
+        unpack(*reinterpret_cast<const uint4*>(row + at), v);
     } else {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        const float4 a = reinterpret_cast<const float4*>(row + at)[0];
+        const float4 b = reinterpret_cast<const float4*>(row + at)[1];
         v[0] = make_float2(a.x, a.y);
         v[1] = make_float2(a.z, a.w);
         v[2] = make_float2(b.x, b.y);
         v[3] = make_float2(b.z, b.w);
     }
 }
-template <typename T>
-__device__ __forceinline__ void to_shared(char* row, int at, const F8& v) {
-    T* p = reinterpret_cast<T*>(row) + at;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) p[k] = from_f<T>(value(v, k));
+
+// Bytes a stage keeps for `share` columns of T: the row's 16-byte units, two of
+// which it may share with its neighbours, and for threads behind the row's end.
+template <typename T, bool VECTOR>
+__host__ __device__ constexpr int stage_part(int share, int lanes) {
+    return VECTOR ? share * (int)sizeof(T) : (lanes * (int)sizeof(T) + 47) / 16 * 16;
 }
-constexpr int kMaxStages = 6;
+
+// One array whose rows come through the ring, in shared memory: a lane of the
+// team's first warp copies them, so that all arrays are copied by the same few
+// instructions.
+struct Feed {
+    const char *next, *lo, *hi;   // the next row's columns; the array's limits
+    int64_t step;                 // bytes from row to row
+    int bytes, at;                // of a row's columns; their place in a stage
+};
+constexpr int kFeeds = 5;   // h, x, grad_n, grad_new, the statistics
+
+// Copies f's next row into the stage and arrives at its barrier.  In bulk go whole
+// 16-byte units, with what the first and last hold of the neighbours (not VECTOR);
+// units that reach out of the array go value by value.
+template <bool VECTOR>
+__device__ __forceinline__ void feed_row(Feed& f, char* stage, void* bar, unsigned long long policy) {
+    const char* from = f.next;
+    f.next = from + f.step;
+    char* to = stage + f.at;
+    if constexpr (VECTOR) {
+        expect_bytes(bar, (unsigned)f.bytes);
+        copy_part(bar, to, from, (unsigned)f.bytes, policy);
+    } else {
+        const int shift = (int)((uintptr_t)from & 15);
+        const char *a = from - shift, *b = from + f.bytes + (-(uintptr_t)(from + f.bytes) & 15);
+        if (a < f.lo) a += 16;
+        if (b > f.hi) b -= 16;
+        if (b < a) b = a;
+        to += shift;   // where `from` goes
+        for (int k = 0; k < min(f.bytes, (int)(a - from)); k += 2)
+            *reinterpret_cast<uint16_t*>(to + k) = *reinterpret_cast<const uint16_t*>(from + k);
+        for (int k = max(0, max((int)(a - from), (int)(b - from))); k < f.bytes; k += 2)
+            *reinterpret_cast<uint16_t*>(to + k) = *reinterpret_cast<const uint16_t*>(from + k);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        const unsigned bytes = (unsigned)(b - a);
+        expect_bytes(bar, bytes);
+        if (bytes > 0) copy_part(bar, to + (a - from), a, bytes, policy);
+    }
+}
 
 // With q = g w1 hh and p = g w1, the gradient u = t p of the normalised block has
 //   sum u hh = sum dx q + r2 (sum e q - m0 sum q - m1 sum xh q)
@@ -527,18 +589,19 @@ constexpr int kMaxStages = 6;
 //
 // FULL: a mean is removed or a bias is there, so sums without the normalised
 // value are needed as well.  GROUPED: the gate differs between rows; its sums go
-// out at the end of every group, weighted into the others.  With one chunk a
-// thread the parameters' gradients stay in registers; with more (rows above 4096
-// columns) they are in shared memory, each value of one thread.
+// out at the end of every group, weighted into the others.
+//
+// Rows of more than 8192 columns: two or four chunks a thread, loaded straight
+// into registers; the parameters' gradients are in shared memory, each value of
+// one thread.
 template <typename XT, typename HT, bool VECTOR, int I, bool FULL, bool GROUPED>
 __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant__
                                                            mdq_residual_norm_grad_desc g,
                                                            const __grid_constant__ Teams G,
                                                            const __grid_constant__ Partials W) {
     constexpr int kLog = FULL ? 4 : 2, kKinds = FULL ? 4 : 2;
-    constexpr bool kRegs = I == 1;
     __shared__ float slots[2 * kSlots * (1 << kLog)];
-    extern __shared__ __align__(16) float shared[];   // [kinds][share] (several teams, or I > 1)
+    extern __shared__ __align__(16) float shared[];   // [kinds][share]
     const mdq_residual_norm_desc& d = g.f;
     Place<VECTOR> P(G, (int)d.dim, slots, kSlots << kLog);
     const Cols<VECTOR>& cols = P.cols;
@@ -553,12 +616,6 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
     const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
     const int c0 = P.R.rank * G.share;
 
-    // The parameters' gradients; with GROUPED the sums of the present group apart.
-    F8 acc[kRegs ? kKinds : 1], group[GROUPED && kRegs ? 2 : 1];
-#pragma unroll
-    for (int j = 0; j < (kRegs ? kKinds : 1); ++j) fill(acc[j], 0.0f);
-#pragma unroll
-    for (int j = 0; j < (GROUPED && kRegs ? 2 : 1); ++j) fill(group[j], 0.0f);
     const auto place_of = [&](int kind, const Cols<VECTOR>& c, int k) {
         return shared + kind * G.share + c.at(k) - c0;
     };
@@ -578,18 +635,10 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
                 if (c.has(k)) *place_of(kind, c, k) += value(v, k);
         }
     };
-    if (!kRegs) {
-        for (int i = threadIdx.x; i < (GROUPED ? 6 : kKinds) * G.share; i += blockDim.x) shared[i] = 0.0f;
-        __syncthreads();
-    }
-    // With one chunk the parameters and a row's values stay in registers between
-    // its two steps, and where the loads of two rows fit as well, the next row is
-    // loaded ahead.
-    constexpr bool kAhead = I * (sizeof(XT) + sizeof(HT)) <= (FULL ? 4 : 6);
-    F8 kp, kb, kw;
-    if (kRegs) parameters(d.pre_weight, pb, cols, 1.0f, kw);
-    GradRaw<XT, HT, VECTOR> next[I];
-    float4 nst = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = threadIdx.x; i < (GROUPED ? 6 : kKinds) * G.share; i += blockDim.x) shared[i] = 0.0f;
+    __syncthreads();
+    GradRaw<XT, HT, VECTOR> raw[I];
+    float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const XT *xr = x + r0 * d.x_stride, *gxr = gx + r0 * g.grad_new_stride;
     const HT *hr = h + r0 * d.h_stride, *gnr = gn + r0 * g.grad_n_stride;
     const float4* sr = reinterpret_cast<const float4*>(d.stats) + r0;
@@ -597,12 +646,12 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             const Cols<VECTOR> c = cols.chunk(i);
-            if (h != nullptr) next[i].h.load(hr, c);
-            next[i].x.load(xr, c);
-            if (gn != nullptr) next[i].gn.load(gnr, c);
-            if (gx != nullptr) next[i].gx.load(gxr, c);
+            if (h != nullptr) raw[i].h.load(hr, c);
+            raw[i].x.load(xr, c);
+            if (gn != nullptr) raw[i].gn.load(gnr, c);
+            if (gx != nullptr) raw[i].gx.load(gxr, c);
         }
-        nst = __ldg(sr++);
+        st = __ldg(sr++);
         xr += d.x_stride;
         hr += d.h_stride;
         gxr += g.grad_new_stride;
@@ -610,40 +659,19 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
     };
     XT* xo = static_cast<XT*>(g.grad_x) + r0 * d.dim;
     HT* ho = static_cast<HT*>(g.grad_h) + r0 * d.dim;
-    if (kAhead && r0 < r1) fetch();
-    int64_t turn = r0;   // the row at which another row of the gate begins
     // The rows of every CTA of a cluster are the same, so all take part in its sums.
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, ho += d.dim) {
-        if (!kAhead) fetch();
-        GradRaw<XT, HT, VECTOR> raw[I];
-#pragma unroll
-        for (int i = 0; i < I; ++i) raw[i] = next[i];
-        const float4 st = nst;
-        if (kAhead && r + 1 < r1) fetch();
+        fetch();
         const void* gate = d.gate;
         if (GROUPED && d.gate_rows > 1)
             gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
-        if (kRegs && r == turn) {
-            fill(kp, 0.0f);
-            if (h != nullptr) post_parameters<FULL>(d, gate, pb, cols, kp, kb);
-            turn = GROUPED ? (r / per + 1) * per : r1;
-        }
-
         // hh, xh, e and p of a chunk; outside of the row e and p are 0
         const auto values = [&](int i, const Cols<VECTOR>& c, F8& hh, F8& xh, F8& e, F8& p) {
             F8 b;
             raw[i].x.get(xh);
             if (h != nullptr) {
                 raw[i].h.get(hh);
-                if constexpr (kRegs) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        p[j] = kp[j];
-                        if (FULL) b[j] = kb[j];
-                    }
-                } else {
-                    post_parameters<FULL>(d, gate, pb, c, p, b);
-                }
+                post_parameters<FULL>(d, gate, pb, c, p, b);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (FULL) hh[j] = add(hh[j], both(-st.x));
@@ -657,12 +685,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
                 fill(p, 0.0f);
             }
             raw[i].gn.get(e);
-            if constexpr (kRegs) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) b[j] = kw[j];
-            } else {
-                parameters(d.pre_weight, pb, c, 1.0f, b);
-            }
+            parameters(d.pre_weight, pb, c, 1.0f, b);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (FULL) xh[j] = add(xh[j], both(-st.z));
@@ -715,7 +738,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
         for (int i = 0; i < I; ++i) {
             const Cols<VECTOR> c = cols.chunk(i);
             F8 t, dn, o;
-            if (!kRegs) values(i, c, hh, xh, e, p);
+            values(i, c, hh, xh, e, p);
             raw[i].gx.get(t);
             raw[i].gn.get(dn);
 #pragma unroll
@@ -723,18 +746,11 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
                 float2 y = fma(xh[j], both(-m1), e[j]);
                 if (FULL) y = add(y, both(-m0));
                 t[j] = fma(both(rx), y, t[j]);
-                if constexpr (kRegs) {
-                    acc[kPre][j] = fma(dn[j], xh[j], acc[kPre][j]);
-                    if (FULL) acc[FULL ? kPreBias : 0][j] = add(acc[FULL ? kPreBias : 0][j], dn[j]);
-                } else {
-                    xh[j] = mul(xh[j], dn[j]);
-                }
+                xh[j] = mul(xh[j], dn[j]);
                 o[j] = mul(both(a), t[j]);
             }
-            if constexpr (!kRegs) {
-                add_to(kPre, c, xh);
-                if (FULL) add_to(kPreBias, c, dn);
-            }
+            add_to(kPre, c, xh);
+            if (FULL) add_to(kPreBias, c, dn);
             store(xo, c, o);
             if (h == nullptr) continue;
 #pragma unroll
@@ -744,23 +760,10 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
                 o[j] = mul(both(st.y), fma(hh[j], both(-u1), o[j]));
             }
             store(ho, c, o);
-            if constexpr (kRegs) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (GROUPED) {
-                        group[0][j] = fma(t[j], hh[j], group[0][j]);
-                        group[1][j] = add(group[1][j], t[j]);
-                    } else {
-                        acc[kPost][j] = fma(t[j], hh[j], acc[kPost][j]);
-                        if (FULL) acc[FULL ? kPostBias : 0][j] = add(acc[FULL ? kPostBias : 0][j], t[j]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) hh[j] = mul(hh[j], t[j]);
-                add_to(GROUPED ? 4 : kPost, c, hh);
-                if (FULL) add_to(GROUPED ? 5 : kPostBias, c, t);
-            }
+            for (int j = 0; j < 4; ++j) hh[j] = mul(hh[j], t[j]);
+            add_to(GROUPED ? 4 : kPost, c, hh);
+            if (FULL) add_to(GROUPED ? 5 : kPostBias, c, t);
         }
         if constexpr (GROUPED) {
             if (r + 1 == r1 || (r + 1) % per == 0) {   // the group ends, or this team's part of it
@@ -777,21 +780,10 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         if (!c.has(k)) continue;
-                        float sum, sum_b;
-                        if constexpr (kRegs) {
-                            sum = value(group[0], k);
-                            sum_b = value(group[GROUPED ? 1 : 0], k);
-                            set(acc[kPost], k, fmaf(value(w, k), sum, value(acc[kPost], k)));
-                            if (FULL)
-                                set(acc[FULL ? kPostBias : 0], k,
-                                    fmaf(value(w, k), sum_b, value(acc[FULL ? kPostBias : 0], k)));
-                        } else {
-                            sum = *place_of(4, c, k);
-                            sum_b = *place_of(5, c, k);
-                            *place_of(kPost, c, k) += value(w, k) * sum;
-                            if (FULL) *place_of(kPostBias, c, k) += value(w, k) * sum_b;
-                            *place_of(4, c, k) = *place_of(5, c, k) = 0.0f;
-                        }
+                        const float sum = *place_of(4, c, k), sum_b = *place_of(5, c, k);
+                        *place_of(kPost, c, k) += value(w, k) * sum;
+                        if (FULL) *place_of(kPostBias, c, k) += value(w, k) * sum_b;
+                        *place_of(4, c, k) = *place_of(5, c, k) = 0.0f;
                         if (whole) {
                             if (g.grad_gate != nullptr)
                                 store_any(g.grad_gate, pb, k0 * d.dim + c.at(k),
@@ -802,50 +794,22 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
                         }
                     }
                 }
-                if (kRegs) {
-                    fill(group[0], 0.0f);
-                    fill(group[GROUPED && kRegs ? 1 : 0], 0.0f);
-                }
             }
         }
     }
     float* out = W.sums + (int64_t)(blockIdx.x / P.R.ctas) * 4 * d.dim;
-    if constexpr (kRegs) {
-        // The CTA's sums: its teams add theirs in turn.
-        for (int i = 0; i < G.teams; ++i) {
-            if (i > 0) __syncthreads();
-            if (P.team != i) continue;
+    __syncthreads();
+    const int mine = max(0, min((int)d.dim - c0, G.share));
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (!cols.has(k)) continue;
-#pragma unroll
-                for (int j = 0; j < kKinds; ++j) {
-                    float* q = place_of(j, cols, k);
-                    const float v = i > 0 ? *q + value(acc[j], k) : value(acc[j], k);
-                    if (i + 1 < G.teams) *q = v;
-                    else out[j * d.dim + cols.at(k)] = v;
-                }
-            }
-        }
-    } else {
-        __syncthreads();
-        const int mine = max(0, min((int)d.dim - c0, G.share));
-#pragma unroll
-        for (int j = 0; j < kKinds; ++j)
-            for (int i = threadIdx.x; i < mine; i += blockDim.x)
-                out[j * d.dim + c0 + i] = shared[j * G.share + i];
-    }
+    for (int j = 0; j < kKinds; ++j)
+        for (int i = threadIdx.x; i < mine; i += blockDim.x)
+            out[j * d.dim + c0 + i] = shared[j * G.share + i];
     if (P.R.ctas > 1) cg::this_cluster().sync();
 }
 
-// Waits for copies that ran out.
-static __device__ unsigned int g_norm_timeouts;
-
-// The same for rows on 16-byte boundaries and many of them: a team's rows come
-// through a ring of `stages` in shared memory by bulk copies that one thread
-// issues ahead, so that no registers hold loads and several rows are on their way
-// at any time.  One chunk of columns a thread; wider rows take a cluster.
-template <typename XT, typename HT, bool FULL, bool GROUPED>
+// The same with the rows in a ring, as in the forward pass, for up to 8192
+// columns: one chunk of columns a thread and one or two CTAs a row.
+template <typename XT, typename HT, bool VECTOR, bool FULL, bool GROUPED>
 __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_constant__
                                                              mdq_residual_norm_grad_desc g,
                                                              const __grid_constant__ Teams G,
@@ -854,63 +818,73 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     constexpr int kLog = FULL ? 4 : 2, kKinds = FULL ? 4 : 2;
     __shared__ float slots[2 * kSlots * (1 << kLog)];
     __shared__ unsigned long long full[kTeam / 32][kMaxStages];
+    __shared__ Feed feeds[kTeam / 32][kFeeds];
     extern __shared__ __align__(16) char ring[];   // [team][stage]: h, x, grad_n, grad_new, stats
     const mdq_residual_norm_desc& d = g.f;
-    Place<true> P(G, (int)d.dim, slots, kSlots << kLog);
-    const Cols<true>& cols = P.cols;
+    Place<VECTOR> P(G, (int)d.dim, slots, kSlots << kLog);
+    const Cols<VECTOR>& cols = P.cols;
     const bool layer = FULL && d.kind == MDQ_NORM_LAYER, pb = d.param_dtype == MDQ_BF16;
     const float inv = 1.0f / (float)d.dim;
     const int64_t per = d.rows / d.gate_rows;
     const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
-    const int c0 = P.R.rank * G.share, mine = max(0, cols.end - c0);
-    const bool has_h = d.h != nullptr, has_gn = g.grad_n != nullptr, has_gx = g.grad_new != nullptr;
+    const int c0 = P.R.rank * G.share, mine = cols.end - c0, lanes = G.threads * 8;
+    const bool has_h = d.h != nullptr, has_gn = g.grad_n != nullptr;
 
-    const int at_x = G.share * (int)sizeof(HT), at_gn = at_x + G.share * (int)sizeof(XT);
-    const int at_gx = at_gn + G.share * (int)sizeof(HT), at_st = at_gx + G.share * (int)sizeof(XT);
-    const int stage_bytes = at_st + 16;
+    const int hb = stage_part<HT, VECTOR>(G.share, lanes), xb = stage_part<XT, VECTOR>(G.share, lanes);
+    const int at_x = hb, at_gn = hb + xb, at_gx = 2 * hb + xb;
+    const int at_st = 2 * (hb + xb), stage_bytes = at_st + 16;
     char* stage0 = ring + (size_t)P.team * stages * stage_bytes;
-    // Threads behind the row's end read its last values; their parameters are 0,
-    // and so is what they add.  An absent array's place holds zeros.
-    const int at = min(8 * P.t, mine - 8);
-    for (int k = 0; k < stages; ++k) {
-        char* q = stage0 + k * stage_bytes;
-        const F8 zero = {};
-        if (!has_h) to_shared<HT>(q, at, zero);
-        if (!has_gn) to_shared<HT>(q + at_gn, at, zero);
-        if (!has_gx) to_shared<XT>(q + at_gx, at, zero);
+    const void* const arrays[kFeeds] = {d.h, d.x, g.grad_n, g.grad_new, d.stats};
+    const int64_t strides[kFeeds] = {d.h_stride, d.x_stride, g.grad_n_stride, g.grad_new_stride, 4};
+    const int parts[kFeeds] = {0, at_x, at_gn, at_gx, at_st};
+    int there = 0;   // arrays that are fed
+#pragma unroll
+    for (int k = 0; k < kFeeds; ++k) {
+        const int size = k == 4 ? 4 : k & 1 ? (int)sizeof(XT) : (int)sizeof(HT);
+        if (P.t == 0) {
+            const char* p = static_cast<const char*>(arrays[k]) + (k == 4 ? 0 : (int64_t)c0 * size);
+            const int64_t step = strides[k] * size;
+            const int bytes = arrays[k] == nullptr ? 0 : k == 4 ? 16 : mine * size;
+            feeds[P.team][k] = {p + r0 * step, p, p + (d.rows - 1) * step + bytes, step, bytes, parts[k]};
+        }
+        there += arrays[k] != nullptr;
+        // An absent array's place holds zeros.
+        if (arrays[k] == nullptr)
+            for (int i = P.t; i < stages * (k & 1 ? xb : hb) / 4; i += G.threads) {
+                const int words = (k & 1 ? xb : hb) / 4;
+                reinterpret_cast<unsigned*>(stage0 + i / words * stage_bytes + parts[k])[i % words] = 0;
+            }
     }
     if (P.t == 0)
-        for (int k = 0; k < stages; ++k) bar_init(&full[P.team][k], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int k = 0; k < stages; ++k) bar_init(&full[P.team][k], there);
+    asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
     if (P.R.ctas > 1) cg::this_cluster().sync();
     else __syncthreads();
 
-    // Copies of the next row into a stage, by the team's first thread.
+    // The next row into the next stage, by the team's first warp.
     const unsigned long long policy = read_once();
-    int64_t ahead = r0;
-    int to = 0;
+    int left = (int)(r1 - r0), to = 0;   // rows to copy
+    const bool feeder = P.t < kFeeds && feeds[P.team][P.t < kFeeds ? P.t : 0].bytes > 0;
     const auto copy_row = [&] {
-        if (ahead >= r1) return;
-        char* s = stage0 + to * stage_bytes;
-        unsigned long long* bar = &full[P.team][to];
-        const unsigned hb = (unsigned)mine * sizeof(HT), xb = (unsigned)mine * sizeof(XT);
-        const auto part = [&](int place, const void* from, unsigned bytes) {
-            copy_part(bar, s + place, from, bytes, policy);
-        };
-        expect_bytes(bar, (has_h ? hb : 0) + xb + (has_gn ? hb : 0) + (has_gx ? xb : 0) + 16);
-        {
-            if (has_h) part(0, static_cast<const HT*>(d.h) + ahead * d.h_stride + c0, hb);
-            part(at_x, static_cast<const XT*>(d.x) + ahead * d.x_stride + c0, xb);
-            if (has_gn) part(at_gn, static_cast<const HT*>(g.grad_n) + ahead * g.grad_n_stride + c0, hb);
-            if (has_gx) part(at_gx, static_cast<const XT*>(g.grad_new) + ahead * g.grad_new_stride + c0, xb);
-        }
-        part(at_st, d.stats + 4 * ahead, 16);
-        ++ahead;
+        if (left == 0) return;
+        if (feeder) feed_row<VECTOR>(feeds[P.team][P.t], stage0 + to * stage_bytes, &full[P.team][to], policy);
+        --left;
         if (++to == stages) to = 0;
     };
-    if (P.t == 0)
+    if (P.R.warp == 0)
         for (int k = 0; k < stages - 1; ++k) copy_row();
 
+    // Threads behind the row's end read its last values (VECTOR) or what lies
+    // there, and drop them.
+    const bool ragged = lanes != mine;
+    const int at = VECTOR ? min(cols.first - c0, mine - 8) : cols.first - c0;
+    // Bytes by which the arrays' rows start behind a 16-byte boundary.
+    unsigned shifts[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int size = k & 1 ? (int)sizeof(XT) : (int)sizeof(HT);
+        shifts[k] = VECTOR ? 0 : (unsigned)((uintptr_t)arrays[k] + (c0 + r0 * strides[k]) * size) & 15;
+    }
     F8 acc[kKinds], group[GROUPED ? 2 : 1], kp, kb, kw;
 #pragma unroll
     for (int j = 0; j < kKinds; ++j) fill(acc[j], 0.0f);
@@ -942,10 +916,18 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
         const float4 st = lost ? make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F)
                                : *reinterpret_cast<const float4*>(s0 + at_st);
         F8 hh, xh, dx, dn;
-        from_shared<XT>(s0 + at_x, at, xh);
-        from_shared<HT>(s0 + at_gn, at, dn);
-        from_shared<XT>(s0 + at_gx, at, dx);
-        from_shared<HT>(s0, at, hh);
+        const HT* gnr = reinterpret_cast<const HT*>(s0 + at_gn + shifts[2]);
+        const XT* gxr = reinterpret_cast<const XT*>(s0 + at_gx + shifts[3]);
+        from_shared<XT, VECTOR>(reinterpret_cast<const XT*>(s0 + at_x + shifts[1]), at, cols.step, xh);
+        from_shared<HT, VECTOR>(gnr, at, cols.step, dn);
+        from_shared<XT, VECTOR>(gxr, at, cols.step, dx);
+        from_shared<HT, VECTOR>(reinterpret_cast<const HT*>(s0 + shifts[0]), at, cols.step, hh);
+        if (ragged) {
+            within_row(xh, cols);
+            within_row(dn, cols);
+            within_row(dx, cols);
+            within_row(hh, cols);
+        }
         float2 s2[FULL ? 10 : 4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -975,7 +957,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
         P.R.template sum<kLog>(s);
         // Every thread is past the row before (a warp alone: in step): its stage is free.
         if (G.threads == 32) __syncwarp();
-        if (P.t == 0 && !lost) copy_row();
+        if (P.R.warp == 0) copy_row();
         const float m1 = s[0] * inv;
         float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(st.w, s[2] - m1 * s[3], s[1]);
         if constexpr (FULL) {
@@ -989,8 +971,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
         const float rx = has_gn ? st.w : 0.0f;
         F8 o;
         if (FULL) {   // read again: the registers were the sums'
-            from_shared<HT>(s0 + at_gn, at, dn);
-            from_shared<XT>(s0 + at_gx, at, dx);
+            from_shared<HT, VECTOR>(gnr, at, cols.step, dn);
+            from_shared<XT, VECTOR>(gxr, at, cols.step, dx);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1023,19 +1005,23 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
                 const int64_t k0 = r / per, first = k0 * per, last = first + per - 1;
                 float* edge = nullptr;
                 if (first < r0 || last >= r1) edge = W.edges + ((P.index * 2 + (first >= r0)) * 2) * d.dim;
-                end_group<true, FULL>(g, gate, pb, cols, k0, edge, group, acc);
+                end_group<VECTOR, FULL>(g, gate, pb, cols, k0, edge, group, acc);
             }
         }
         if (++stage == stages) {
             stage = 0;
             phase ^= 1;
         }
+        if (!VECTOR)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                shifts[k] = (shifts[k] + (unsigned)strides[k] * (k & 1 ? sizeof(XT) : sizeof(HT))) & 15;
     }
     if (lost && P.t == 0)   // copies still on their way end before the CTA does
-        for (int64_t k = ahead - min(ahead - r0, (int64_t)stages); k < ahead; ++k)
-            bar_wait(&full[P.team][(k - r0) % stages], (unsigned)((k - r0) / stages) & 1);
+        for (int64_t k = max((int64_t)0, r1 - r0 - stages); k < r1 - r0; ++k)
+            bar_wait(&full[P.team][k % stages], (unsigned)(k / stages) & 1);
     __syncthreads();
-    end_sums<true, kKinds>(P, G, W, (int)d.dim, reinterpret_cast<float*>(ring), acc);
+    end_sums<VECTOR, kKinds>(P, G, W, (int)d.dim, reinterpret_cast<float*>(ring), acc);
     if (P.R.ctas > 1) cg::this_cluster().sync();
 }
 
@@ -1052,16 +1038,16 @@ cudaError_t run_forward(const mdq_residual_norm_desc& d, const Teams& G, int chu
     return launch(k, dim3(grid), G.threads * G.teams, 0, stream, cluster, false, d, G);
 }
 
-template <typename XT, typename HT>
+template <typename XT, typename HT, bool VECTOR>
 cudaError_t run_stream(const mdq_residual_norm_grad_desc& g, const Teams& G, const Partials& W,
                        int stages, size_t smem, int grid, int cluster, bool full, bool grouped,
                        cudaStream_t stream) {
     typedef void (*Kernel)(const mdq_residual_norm_grad_desc, const Teams, const Partials, int);
-    const Kernel k = full ? (grouped ? (Kernel)norm_grad_stream<XT, HT, true, true>
-                                     : (Kernel)norm_grad_stream<XT, HT, true, false>)
-                          : (grouped ? (Kernel)norm_grad_stream<XT, HT, false, true>
-                                     : (Kernel)norm_grad_stream<XT, HT, false, false>);
-    return launch<209 * 1024>(k, dim3(grid), G.threads * G.teams, smem, stream, cluster, false, g, G, W,
+    const Kernel k = full ? (grouped ? (Kernel)norm_grad_stream<XT, HT, VECTOR, true, true>
+                                     : (Kernel)norm_grad_stream<XT, HT, VECTOR, true, false>)
+                          : (grouped ? (Kernel)norm_grad_stream<XT, HT, VECTOR, false, true>
+                                     : (Kernel)norm_grad_stream<XT, HT, VECTOR, false, false>);
+    return launch<205 * 1024>(k, dim3(grid), G.threads * G.teams, smem, stream, cluster, false, g, G, W,
                               stages);
 }
 
@@ -1069,17 +1055,12 @@ template <typename XT, typename HT, bool VECTOR>
 cudaError_t run_backward(const mdq_residual_norm_grad_desc& g, const Teams& G, const Partials& W,
                          int chunks, int grid, int cluster, bool full, bool grouped,
                          cudaStream_t stream) {
-    const int kinds = chunks > 1 ? (grouped ? 6 : full ? 4 : 2) : G.teams > 1 ? (full ? 4 : 2) : 0;
+    const int kinds = grouped ? 6 : full ? 4 : 2;
     typedef void (*Kernel)(const mdq_residual_norm_grad_desc, const Teams, const Partials);
-    const Kernel k =
-        chunks == 1 ? (full ? (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, true, true>
-                                       : (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, true, false>)
-                            : (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, false, true>
-                                       : (Kernel)norm_grad_rows<XT, HT, VECTOR, 1, false, false>))
-        : chunks == 2 ? (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, true, true>
-                         : full  ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, true, false>
-                                 : (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, false, false>)
-                      : (Kernel)norm_grad_rows<XT, HT, VECTOR, 4, false, false>;
+    const Kernel k = chunks == 2 ? (grouped ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, true, true>
+                                    : full  ? (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, true, false>
+                                            : (Kernel)norm_grad_rows<XT, HT, VECTOR, 2, false, false>)
+                                 : (Kernel)norm_grad_rows<XT, HT, VECTOR, 4, false, false>;
     return launch<210 * 1024>(k, dim3(grid), G.threads * G.teams, sizeof(float) * kinds * G.share,
                               stream, cluster, false, g, G, W);
 }
@@ -1093,7 +1074,7 @@ cudaError_t run_backward(const mdq_residual_norm_grad_desc& g, const Teams& G, c
     cudaError_t backward_##S(const mdq_residual_norm_grad_desc&, const Teams&, const Partials&,    \
                              int, int, int, bool, bool, bool, cudaStream_t);                       \
     cudaError_t stream_##S(const mdq_residual_norm_grad_desc&, const Teams&, const Partials&, int, \
-                           size_t, int, int, bool, bool, cudaStream_t);
+                           size_t, int, int, bool, bool, bool, cudaStream_t);
 MDQ_NORM_TYPES(MDQ_NORM_DECLARE)
 
 // The kernels of one pair of types (x, h), in a file of its own.
@@ -1113,9 +1094,12 @@ MDQ_NORM_TYPES(MDQ_NORM_DECLARE)
                                                     stream);                                       \
     }                                                                                              \
     cudaError_t stream_##S(const mdq_residual_norm_grad_desc& g, const Teams& G, const Partials& W,\
-                           int stages, size_t smem, int grid, int cluster, bool full,              \
+                           int stages, size_t smem, int grid, int cluster, bool vector, bool full, \
                            bool grouped, cudaStream_t stream) {                                    \
-        return run_stream<XT, HT>(g, G, W, stages, smem, grid, cluster, full, grouped, stream);    \
+        return vector ? run_stream<XT, HT, true>(g, G, W, stages, smem, grid, cluster, full,       \
+                                                 grouped, stream)                                  \
+                      : run_stream<XT, HT, false>(g, G, W, stages, smem, grid, cluster, full,      \
+                                                  grouped, stream);                                \
     }                                                                                              \
     }
 

@@ -158,7 +158,9 @@ constexpr int kMaxShared = 223 * 1024;
 template <int MOST = kMaxShared, typename... P, typename... A>
 inline cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
                           cudaStream_t stream, int cluster, bool dependent, A... args) {
-    if (smem > 48 * 1024) {   // always the same limit: calls of other threads may set it as well
+    // (48 KB with the static arrays need no leave.)  Always the same limit: calls
+    // of other threads may set it as well.
+    if (smem > 16 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(
             reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
             MOST);
