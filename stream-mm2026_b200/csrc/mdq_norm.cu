@@ -307,22 +307,38 @@ bool plan_ring(int64_t rows, int64_t stage, bool one, Teams* G, int* stages, siz
     return true;
 }
 
+struct RowsPlan {
+    Teams G;
+    int cluster, chunks, grid;
+    int stages;        // of the kernel with a ring, 0: the other
+    size_t smem;
+};
 // Forward: two chunks a thread for many rows above 256 columns, one for narrow
 // or few (as few threads as 512 allow), four where that is not enough.
 // 32768 bf16 rows of 768 / 128 columns: 48 / 18 us with two chunks, 108 / 15 with one.
-bool plan_forward(int64_t rows, int64_t dim, int* cluster, int* chunks, Teams* G, int* grid) {
-    if (!plan_columns(dim, 4, cluster, G)) return false;
-    *chunks = rows > 296 && G->share > 256 ? 2 : 1;
-    while (threads_for(G->share, *chunks) > kTeam) *chunks *= 2;
-    G->threads = threads_for(G->share, *chunks);
-    G->teams = *cluster > 1 || G->threads > 64 ? 1 : 128 / G->threads;
-    // 512 threads an SM, as their registers go.
-    const int64_t ctas = G->threads * G->teams >= kTeam ? 1 : kTeam / (G->threads * G->teams);
-    const int64_t need = ceil_div(rows, G->teams), most = 148 * ctas / *cluster;
-    *grid = (int)(need < most ? need : most);
-    G->run = (int)ceil_div(rows, (int64_t)*grid * G->teams);
-    *grid *= *cluster;
-    return true;
+bool plan_forward(int64_t rows, int64_t dim, int64_t row_bytes, bool vec, bool ring, RowsPlan* p) {
+    for (int most = 4; most >= 1; most /= 2) {
+        if (!plan_columns(dim, most, &p->cluster, &p->G)) return false;
+        Teams& G = p->G;
+        p->chunks = rows > 296 && G.share > 256 && most > 1 ? 2 : 1;
+        while (threads_for(G.share, p->chunks) > kTeam) p->chunks *= 2;
+        G.threads = threads_for(G.share, p->chunks);
+        p->stages = 0;
+        int64_t ctas = 1;   // of an SM: 512 threads, as their registers go
+        if (!ring) {
+            G.teams = p->cluster > 1 || G.threads > 64 ? 1 : 128 / G.threads;
+            if (G.threads * G.teams < kTeam) ctas = kTeam / (G.threads * G.teams);
+        } else if (!plan_ring(rows, stage_of(row_bytes, 2, vec, G, p->chunks), p->cluster > 1, &G,
+                              &p->stages, &p->smem)) {
+            continue;   // a stage too large: more CTAs a row
+        }
+        const int64_t need = ceil_div(rows, G.teams), all = 148 * ctas / p->cluster;
+        p->grid = (int)(need < all ? need : all);
+        G.run = (int)ceil_div(rows, (int64_t)p->grid * G.teams);
+        p->grid *= p->cluster;
+        return true;
+    }
+    return false;
 }
 
 // The backward pass's teams, their rows, and what the workspace holds.
@@ -425,15 +441,13 @@ mdq_status mdq_residual_norm(const mdq_residual_norm_desc* d, cudaStream_t strea
     mdq_residual_norm_desc a = *d;
     if (a.pre_weight == nullptr) a.n = nullptr;
     if (!aligned16(a.stats)) return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm: stats misaligned");
-    Teams G = {};
-    int cluster = 1, chunks = 1, grid = 1;
-    if (plan_forward(a.rows, a.dim, &cluster, &chunks, &G, &grid)) {
-        const bool vec = vector_rows(a) && aligned16(a.x_new) && aligned16(a.n);
-        const bool full = a.kind == MDQ_NORM_LAYER || a.post_bias != nullptr || a.pre_bias != nullptr;
-        return status_of(MDQ_NORM_PICK(forward, a.x_dtype, a.h_dtype)(a, G, chunks, grid, cluster, vec,
-                                                                      full, stream),
+    RowsPlan p;
+    const bool vec = vector_rows(a) && aligned16(a.x_new) && aligned16(a.n);
+    const bool full = a.kind == MDQ_NORM_LAYER || a.post_bias != nullptr || a.pre_bias != nullptr;
+    if (plan_forward(a.rows, a.dim, type_size(a.x_dtype) + type_size(a.h_dtype), vec, full || !vec, &p))
+        return status_of(MDQ_NORM_PICK(forward, a.x_dtype, a.h_dtype)(
+                             a, p.G, p.chunks, p.grid, p.cluster, p.stages, p.smem, vec, full, stream),
                          "residual norm");
-    }
     norm_wide<<<(unsigned)d->rows, kThreads, 0, stream>>>(a);
     return launch_status("residual norm");
 }

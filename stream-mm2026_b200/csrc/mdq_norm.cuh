@@ -283,6 +283,157 @@ struct Place {
     }
 };
 
+// ---------------------------------------------------------- rows in a ring
+
+constexpr int kMaxStages = 6;
+
+// Waits for copies that ran out.
+static __device__ unsigned int g_norm_timeouts;
+
+// A chunk's eight values in shared memory, the row's first at `row`.
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void from_shared(const T* row, int at, int step, F8& v) {
+    if constexpr (!VECTOR) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) set(v, k, to_f(row[at + k * step]));
+    } else if constexpr (sizeof(T) == 2) {
+        unpack(*reinterpret_cast<const uint4*>(row + at), v);
+    } else {
+        const float4 a = reinterpret_cast<const float4*>(row + at)[0];
+        const float4 b = reinterpret_cast<const float4*>(row + at)[1];
+        v[0] = make_float2(a.x, a.y);
+        v[1] = make_float2(a.z, a.w);
+        v[2] = make_float2(b.x, b.y);
+        v[3] = make_float2(b.z, b.w);
+    }
+}
+
+// Bytes a stage keeps for `share` columns of T: the row's 16-byte units, two of
+// which it may share with its neighbours, and for threads behind the row's end.
+template <typename T, bool VECTOR>
+__host__ __device__ constexpr int stage_part(int share, int lanes) {
+    return VECTOR ? share * (int)sizeof(T) : (lanes * (int)sizeof(T) + 47) / 16 * 16;
+}
+
+// One array whose rows come through the ring, in shared memory: a lane of the
+// team's first warp copies them, so that all arrays are copied by the same few
+// instructions.
+struct Feed {
+    const char *next, *lo, *hi;   // the next row's columns; the array's limits
+    int64_t step;                 // bytes from row to row
+    int bytes, at;                // of a row's columns; their place in a stage
+};
+constexpr int kFeeds = 5;   // h, x, grad_n, grad_new, the statistics
+
+// Copies f's next row into the stage and arrives at its barrier.  In bulk go whole
+// 16-byte units, with what the first and last hold of the neighbours (not VECTOR);
+// units that reach out of the array go value by value.
+template <bool VECTOR>
+__device__ __forceinline__ void feed_row(Feed& f, char* stage, void* bar, unsigned long long policy) {
+    const char* from = f.next;
+    f.next = from + f.step;
+    char* to = stage + f.at;
+    if constexpr (VECTOR) {
+        expect_bytes(bar, (unsigned)f.bytes);
+        copy_part(bar, to, from, (unsigned)f.bytes, policy);
+    } else {
+        const int shift = (int)((uintptr_t)from & 15);
+        const char *a = from - shift, *b = from + f.bytes + (-(uintptr_t)(from + f.bytes) & 15);
+        if (a < f.lo) a += 16;
+        if (b > f.hi) b -= 16;
+        if (b < a) b = a;
+        to += shift;   // where `from` goes
+        for (int k = 0; k < min(f.bytes, (int)(a - from)); k += 2)
+            *reinterpret_cast<uint16_t*>(to + k) = *reinterpret_cast<const uint16_t*>(from + k);
+        for (int k = max(0, max((int)(a - from), (int)(b - from))); k < f.bytes; k += 2)
+            *reinterpret_cast<uint16_t*>(to + k) = *reinterpret_cast<const uint16_t*>(from + k);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        const unsigned bytes = (unsigned)(b - a);
+        expect_bytes(bar, bytes);
+        if (bytes > 0) copy_part(bar, to + (a - from), a, bytes, policy);
+    }
+}
+
+// A team's ring of rows: its stages, its feeds and the place it is at.
+template <bool VECTOR>
+struct Ring {
+    char* stage0;
+    unsigned long long* full;
+    Feed* feeds;
+    int stages, stage_bytes, left, to, stage;
+    unsigned phase;
+    bool feeder, lost;
+    unsigned long long policy;
+
+    // Before the first barrier of the CTA, by every thread of the team.
+    // arrays[k] with strides[k] elements of sizes[k] bytes a row; parts[k]: the place
+    // of its `mine` columns in a stage; the last array is 16 bytes a row (`tail`).
+    template <int N>
+    __device__ __forceinline__ void open(const void* const (&arrays)[N], const int64_t (&strides)[N],
+                                         const int (&sizes)[N], const int (&parts)[N + 1], bool tail,
+                                         int c0, int mine, int64_t rows, int64_t r0, int64_t r1, int t,
+                                         int threads) {
+        int there = 0;   // arrays that are fed
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const bool whole = tail && k == N - 1;
+            if (t == 0) {
+                const char* p = static_cast<const char*>(arrays[k]) + (whole ? 0 : (int64_t)c0 * sizes[k]);
+                const int64_t step = strides[k] * sizes[k];
+                const int bytes = arrays[k] == nullptr ? 0 : whole ? 16 : mine * sizes[k];
+                feeds[k] = {p + r0 * step, p, p + (rows - 1) * step + bytes, step, bytes, parts[k]};
+            }
+            there += arrays[k] != nullptr;
+            const int words = (parts[k + 1] - parts[k]) / 4;
+            if (arrays[k] == nullptr)   // its place holds zeros
+                for (int i = t; i < stages * words; i += threads)
+                    reinterpret_cast<unsigned*>(stage0 + i / words * stage_bytes + parts[k])[i % words] = 0;
+        }
+        if (t == 0)
+            for (int k = 0; k < stages; ++k) bar_init(&full[k], there);
+        asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+        left = (int)(r1 - r0);
+        to = stage = 0;
+        phase = 0;
+        lost = false;
+        policy = read_once();
+    }
+    // Behind that barrier, by the team's first warp: the next row into the next stage.
+    __device__ __forceinline__ void copy_row(int t) {
+        if (left == 0) return;
+        if (feeder) feed_row<VECTOR>(feeds[t], stage0 + to * stage_bytes, &full[to], policy);
+        --left;
+        if (++to == stages) to = 0;
+    }
+    template <int N>
+    __device__ __forceinline__ void start(int t) {
+        feeder = t < N && feeds[t < N ? t : 0].bytes > 0;
+        if (t < 32)
+            for (int k = 0; k < stages - 1; ++k) copy_row(t);
+    }
+    // The present row's stage, once it is there; after a wait that ran out the
+    // results are made NaN (`lost`).
+    __device__ __forceinline__ const char* row(int t) {
+        if (!lost && !bar_wait(&full[stage], phase)) {
+            lost = true;
+            if (t == 0) atomicAdd(&g_norm_timeouts, 1u);
+        }
+        return stage0 + stage * stage_bytes;
+    }
+    __device__ __forceinline__ void next() {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    // Copies still on their way end before the CTA does.
+    __device__ __forceinline__ void close(int t, int64_t rows) {
+        if (lost && t == 0)
+            for (int64_t k = max((int64_t)0, rows - stages); k < rows; ++k)
+                bar_wait(&full[k % stages], (unsigned)(k / stages) & 1);
+    }
+};
+
 // Mean and 1 / deviation of a row (mean 0 without `layer`); its values lose
 // their mean.
 template <int I, bool VECTOR>
@@ -311,35 +462,32 @@ __device__ __forceinline__ float2 statistics(Reducer& R, const Cols<VECTOR>& col
     return make_float2(mean, 1.0f / sqrtf(fmaf(q[0], inv, eps)));
 }
 
-// I chunks of 8 columns a thread.  With one or two, the parameters stay in
-// registers over a team's rows and the next row is loaded ahead (not where twice
-// as many parameters take the registers); with four (rows above 8192 columns)
-// neither fits, and a row is long enough to fill the time.
-// FULL: layer norm or biases.
-template <typename XT, typename HT, bool VECTOR, int I, bool FULL>
+// RMS norm without biases, rows on 16-byte boundaries: rows go straight to
+// registers, I chunks of 8 columns a thread.  With one or two, the parameters stay
+// in registers over a team's rows and the next row is loaded ahead; with four (rows
+// above 8192 columns) neither fits, and a row is long enough to fill the time.
+// 16384 bf16 rows of 4096: 102 us (5.3 TB/s), against 110 through the ring.
+template <typename XT, typename HT, int I>
 __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ mdq_residual_norm_desc d,
                                                       const __grid_constant__ Teams G) {
     __shared__ float slots[2 * kSlots];
-    Place<VECTOR> P(G, (int)d.dim, slots, kSlots);
-    const Cols<VECTOR>& cols = P.cols;
+    Place<true> P(G, (int)d.dim, slots, kSlots);
+    const Cols<true>& cols = P.cols;
     if (P.R.ctas > 1) cg::this_cluster().sync();   // all run before their memory is written to
-    const bool layer = FULL && d.kind == MDQ_NORM_LAYER, pb = d.param_dtype == MDQ_BF16;
+    const bool pb = d.param_dtype == MDQ_BF16;
     const float inv = 1.0f / (float)d.dim;
     const XT* x = static_cast<const XT*>(d.x);
     const HT* h = static_cast<const HT*>(d.h);
     const int64_t per = d.rows / d.gate_rows;
     const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
-    constexpr bool kKeep = I <= 2, kAhead = kKeep && !(FULL && I == 2);
-    F8 kp[kKeep ? I : 1], kb[kKeep && FULL ? I : 1], kw[kKeep ? I : 1], kc[kKeep && FULL ? I : 1];
+    constexpr bool kKeep = I <= 2;
+    F8 kp[kKeep ? I : 1], kw[kKeep ? I : 1], none;
     if constexpr (kKeep) {
 #pragma unroll
-        for (int i = 0; i < I; ++i) {
-            parameters(d.pre_weight, pb, cols.chunk(i), 1.0f, kw[i]);
-            if (FULL) parameters(d.pre_bias, pb, cols.chunk(i), 0.0f, kc[FULL ? i : 0]);
-        }
+        for (int i = 0; i < I; ++i) parameters(d.pre_weight, pb, cols.chunk(i), 1.0f, kw[i]);
     }
-    Raw<XT, VECTOR> nx[I];
-    Raw<HT, VECTOR> nh[I];
+    Raw<XT, true> nx[I];
+    Raw<HT, true> nh[I];
     const XT* xr = x + r0 * d.x_stride;
     const HT* hr = h + r0 * d.h_stride;
     const auto fetch = [&] {   // the next row
@@ -353,7 +501,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
     };
     XT* xo = static_cast<XT*>(d.x_new) + r0 * d.dim;
     HT* no = static_cast<HT*>(d.n) + r0 * d.dim;
-    if (kAhead && r0 < r1) fetch();
+    if (kKeep && r0 < r1) fetch();
     int64_t turn = r0;   // the row at which another row of the gate begins
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, no += d.dim) {
         const void* gate = d.gate;
@@ -363,22 +511,155 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
             if (h != nullptr)
 #pragma unroll
                 for (int i = 0; i < I; ++i)
-                    post_parameters<FULL>(d, gate, pb, cols.chunk(i), kp[kKeep ? i : 0],
-                                          kb[kKeep && FULL ? i : 0]);
+                    post_parameters<false>(d, gate, pb, cols.chunk(i), kp[kKeep ? i : 0], none);
             turn = d.gate_rows > 1 ? (r / per + 1) * per : r1;
         }
         F8 v[I];
-        Raw<XT, VECTOR> rx[I];
+        Raw<XT, true> rx[I];
         float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (!kAhead) fetch();
+        if (!kKeep) fetch();
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             rx[i] = nx[i];
             nh[i].get(v[i]);
         }
-        if (kAhead && r + 1 < r1) fetch();
+        if (kKeep && r + 1 < r1) fetch();
         if (h != nullptr) {
-            const float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
+            st.y = statistics<I>(P.R, cols, v, false, inv, d.eps).y;
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const Cols<true> c = cols.chunk(i);
+                F8 p, xv;
+                if constexpr (kKeep) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = kp[i][j];
+                } else {
+                    post_parameters<false>(d, gate, pb, c, p, none);
+                }
+                rx[i].get(xv);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[i][j] = fma(both(d.residual_scale), xv[j], mul(mul(v[i][j], both(st.y)), p[j]));
+                store(xo, c, v[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < I; ++i) rx[i].get(v[i]);
+        }
+        if (d.n != nullptr) {
+            st.w = statistics<I>(P.R, cols, v, false, inv, d.eps).y;
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const Cols<true> c = cols.chunk(i);
+                F8 w;
+                if constexpr (kKeep) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = kw[i][j];
+                } else {
+                    parameters(d.pre_weight, pb, c, 1.0f, w);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][j] = mul(mul(v[i][j], both(st.w)), w[j]);
+                store(no, c, v[i]);
+            }
+        }
+        if (d.stats != nullptr && P.t == 0 && P.R.rank == 0)
+            reinterpret_cast<float4*>(d.stats)[r] = st;
+    }
+    if (P.R.ctas > 1) cg::this_cluster().sync();   // none ends while its memory may be written to
+}
+
+// Layer norm, biases, or rows of any alignment: a team's rows come through a ring
+// of `stages` in shared memory, so that no registers hold loads.  FULL: layer norm
+// or biases.  4096 bf16 rows of 8192, layer norm: 93 us against 115 with rows in
+// registers; 16368 rows of 1601: 93 against 190.
+template <typename XT, typename HT, bool VECTOR, int I, bool FULL>
+__global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant__
+                                                           mdq_residual_norm_desc d,
+                                                           const __grid_constant__ Teams G, int stages) {
+    __shared__ float slots[2 * kSlots];
+    __shared__ unsigned long long full[kTeam / 32][kMaxStages];
+    __shared__ Feed feeds[kTeam / 32][2];
+    extern __shared__ __align__(16) char memory[];   // [team][stage]: h, x
+    Place<VECTOR> P(G, (int)d.dim, slots, kSlots);
+    const Cols<VECTOR>& cols = P.cols;
+    const bool layer = FULL && d.kind == MDQ_NORM_LAYER, pb = d.param_dtype == MDQ_BF16;
+    const float inv = 1.0f / (float)d.dim;
+    const bool has_h = d.h != nullptr;
+    const int64_t per = d.rows / d.gate_rows;
+    const int64_t r0 = min(d.rows, P.index * G.run), r1 = min(d.rows, r0 + G.run);
+    const int c0 = P.R.rank * G.share, mine = cols.end - c0, lanes = G.threads * 8 * I;
+    const int hb = stage_part<HT, VECTOR>(G.share, lanes), xb = stage_part<XT, VECTOR>(G.share, lanes);
+    const void* const arrays[2] = {d.h, d.x};
+    const int64_t strides[2] = {d.h_stride, d.x_stride};
+    constexpr int sizes[2] = {sizeof(HT), sizeof(XT)};
+    const int parts[3] = {0, hb, hb + xb};
+    Ring<VECTOR> ring;
+    ring.stage0 = memory + (size_t)P.team * stages * (hb + xb);
+    ring.full = full[P.team];
+    ring.feeds = feeds[P.team];
+    ring.stages = stages;
+    ring.stage_bytes = hb + xb;
+    ring.open(arrays, strides, sizes, parts, false, c0, mine, d.rows, r0, r1, P.t, G.threads);
+    if (P.R.ctas > 1) cg::this_cluster().sync();   // all run before their memory is written to
+    else __syncthreads();
+    ring.template start<2>(P.t);
+
+    constexpr bool kKeep = I <= 2;
+    F8 kp[kKeep ? I : 1], kb[kKeep && FULL ? I : 1], kw[kKeep ? I : 1], kc[kKeep && FULL ? I : 1];
+    if constexpr (kKeep) {
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            parameters(d.pre_weight, pb, cols.chunk(i), 1.0f, kw[i]);
+            if (FULL) parameters(d.pre_bias, pb, cols.chunk(i), 0.0f, kc[FULL ? i : 0]);
+        }
+    }
+    // Threads behind the row's end read its last values (VECTOR) or what lies
+    // there, and drop them.
+    const bool ragged = lanes != mine;
+    const auto place = [&](int i) {
+        const int at = cols.chunk(i).first - c0;
+        return VECTOR ? min(at, mine - 8) : at;
+    };
+    unsigned shifts[2];   // bytes by which the rows start behind a 16-byte boundary
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        shifts[k] = VECTOR ? 0 : (unsigned)((uintptr_t)arrays[k] + (c0 + r0 * strides[k]) * sizes[k]) & 15;
+    XT* xo = static_cast<XT*>(d.x_new) + r0 * d.dim;
+    HT* no = static_cast<HT*>(d.n) + r0 * d.dim;
+    int64_t turn = r0;   // the row at which another row of the gate begins
+    for (int64_t r = r0; r < r1; ++r, xo += d.dim, no += d.dim) {
+        const void* gate = d.gate;
+        if (gate != nullptr && d.gate_rows > 1 && (!kKeep || r == turn))
+            gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
+        if (kKeep && r == turn) {
+            if (has_h)
+#pragma unroll
+                for (int i = 0; i < I; ++i)
+                    post_parameters<FULL>(d, gate, pb, cols.chunk(i), kp[kKeep ? i : 0],
+                                          kb[kKeep && FULL ? i : 0]);
+            turn = d.gate_rows > 1 ? (r / per + 1) * per : r1;
+        }
+        const char* s0 = ring.row(P.t);
+        const HT* hr = reinterpret_cast<const HT*>(s0 + shifts[0]);
+        const XT* xr = reinterpret_cast<const XT*>(s0 + hb + shifts[1]);
+        F8 v[I];
+        float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        // The first sums of a row end with every thread past the row before, whose
+        // stage is free then.
+        const auto refill = [&] {
+            if (G.threads == 32) __syncwarp();
+            if (P.R.warp == 0) ring.copy_row(P.t);
+        };
+        if (has_h) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                from_shared<HT, VECTOR>(hr, place(i), cols.step, v[i]);
+                if (ragged) within_row(v[i], cols.chunk(i));
+            }
+            float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
+            refill();
+            if (ring.lost) s.y = CUDART_NAN_F;
             st.x = s.x;
             st.y = s.y;
 #pragma unroll
@@ -394,7 +675,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
                 } else {
                     post_parameters<FULL>(d, gate, pb, c, p, b);
                 }
-                rx[i].get(xv);
+                from_shared<XT, VECTOR>(xr, place(i), cols.step, xv);
+                if (ragged) within_row(xv, c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[i][j] = mul(v[i][j], both(s.y));
@@ -406,10 +688,15 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < I; ++i) rx[i].get(v[i]);
+            for (int i = 0; i < I; ++i) {
+                from_shared<XT, VECTOR>(xr, place(i), cols.step, v[i]);
+                if (ragged) within_row(v[i], cols.chunk(i));
+            }
         }
         if (d.n != nullptr) {
-            const float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
+            float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
+            if (!has_h) refill();
+            if (ring.lost) s.y = CUDART_NAN_F;
             st.z = s.x;
             st.w = s.y;
 #pragma unroll
@@ -437,7 +724,12 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
         }
         if (d.stats != nullptr && P.t == 0 && P.R.rank == 0)
             reinterpret_cast<float4*>(d.stats)[r] = st;
+        ring.next();
+        if (!VECTOR)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) shifts[k] = (shifts[k] + (unsigned)strides[k] * sizes[k]) & 15;
     }
+    ring.close(P.t, r1 - r0);
     if (P.R.ctas > 1) cg::this_cluster().sync();   // none ends while its memory may be written to
 }
 
@@ -508,77 +800,6 @@ __device__ __forceinline__ void end_sums(const Place<VECTOR>& P, const Teams& G,
                 else out[(int64_t)j * dim + P.cols.at(k)] = v;
             }
         }
-    }
-}
-
-// ---------------------------------------------------------- rows in a ring
-
-constexpr int kMaxStages = 6;
-
-// Waits for copies that ran out.
-static __device__ unsigned int g_norm_timeouts;
-
-// A chunk's eight values in shared memory, the row's first at `row`.
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void from_shared(const T* row, int at, int step, F8& v) {
-    if constexpr (!VECTOR) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) set(v, k, to_f(row[at + k * step]));
-    } else if constexpr (sizeof(T) == 2) {
-        unpack(*reinterpret_cast<const uint4*>(row + at), v);
-    } else {
-        const float4 a = reinterpret_cast<const float4*>(row + at)[0];
-        const float4 b = reinterpret_cast<const float4*>(row + at)[1];
-        v[0] = make_float2(a.x, a.y);
-        v[1] = make_float2(a.z, a.w);
-        v[2] = make_float2(b.x, b.y);
-        v[3] = make_float2(b.z, b.w);
-    }
-}
-
-// Bytes a stage keeps for `share` columns of T: the row's 16-byte units, two of
-// which it may share with its neighbours, and for threads behind the row's end.
-template <typename T, bool VECTOR>
-__host__ __device__ constexpr int stage_part(int share, int lanes) {
-    return VECTOR ? share * (int)sizeof(T) : (lanes * (int)sizeof(T) + 47) / 16 * 16;
-}
-
-// One array whose rows come through the ring, in shared memory: a lane of the
-// team's first warp copies them, so that all arrays are copied by the same few
-// instructions.
-struct Feed {
-    const char *next, *lo, *hi;   // the next row's columns; the array's limits
-    int64_t step;                 // bytes from row to row
-    int bytes, at;                // of a row's columns; their place in a stage
-};
-constexpr int kFeeds = 5;   // h, x, grad_n, grad_new, the statistics
-
-// Copies f's next row into the stage and arrives at its barrier.  In bulk go whole
-// 16-byte units, with what the first and last hold of the neighbours (not VECTOR);
-// units that reach out of the array go value by value.
-template <bool VECTOR>
-__device__ __forceinline__ void feed_row(Feed& f, char* stage, void* bar, unsigned long long policy) {
-    const char* from = f.next;
-    f.next = from + f.step;
-    char* to = stage + f.at;
-    if constexpr (VECTOR) {
-        expect_bytes(bar, (unsigned)f.bytes);
-        copy_part(bar, to, from, (unsigned)f.bytes, policy);
-    } else {
-        const int shift = (int)((uintptr_t)from & 15);
-        const char *a = from - shift, *b = from + f.bytes + (-(uintptr_t)(from + f.bytes) & 15);
-        if (a < f.lo) a += 16;
-        if (b > f.hi) b -= 16;
-        if (b < a) b = a;
-        to += shift;   // where `from` goes
-        for (int k = 0; k < min(f.bytes, (int)(a - from)); k += 2)
-            *reinterpret_cast<uint16_t*>(to + k) = *reinterpret_cast<const uint16_t*>(from + k);
-        for (int k = max(0, max((int)(a - from), (int)(b - from))); k < f.bytes; k += 2)
-            *reinterpret_cast<uint16_t*>(to + k) = *reinterpret_cast<const uint16_t*>(from + k);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        const unsigned bytes = (unsigned)(b - a);
-        expect_bytes(bar, bytes);
-        if (bytes > 0) copy_part(bar, to + (a - from), a, bytes, policy);
     }
 }
 
@@ -819,7 +1040,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     __shared__ float slots[2 * kSlots * (1 << kLog)];
     __shared__ unsigned long long full[kTeam / 32][kMaxStages];
     __shared__ Feed feeds[kTeam / 32][kFeeds];
-    extern __shared__ __align__(16) char ring[];   // [team][stage]: h, x, grad_n, grad_new, stats
+    extern __shared__ __align__(16) char memory[];   // [team][stage]: h, x, grad_n, grad_new, stats
     const mdq_residual_norm_desc& d = g.f;
     Place<VECTOR> P(G, (int)d.dim, slots, kSlots << kLog);
     const Cols<VECTOR>& cols = P.cols;
@@ -833,46 +1054,20 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     const int hb = stage_part<HT, VECTOR>(G.share, lanes), xb = stage_part<XT, VECTOR>(G.share, lanes);
     const int at_x = hb, at_gn = hb + xb, at_gx = 2 * hb + xb;
     const int at_st = 2 * (hb + xb), stage_bytes = at_st + 16;
-    char* stage0 = ring + (size_t)P.team * stages * stage_bytes;
     const void* const arrays[kFeeds] = {d.h, d.x, g.grad_n, g.grad_new, d.stats};
     const int64_t strides[kFeeds] = {d.h_stride, d.x_stride, g.grad_n_stride, g.grad_new_stride, 4};
-    const int parts[kFeeds] = {0, at_x, at_gn, at_gx, at_st};
-    int there = 0;   // arrays that are fed
-#pragma unroll
-    for (int k = 0; k < kFeeds; ++k) {
-        const int size = k == 4 ? 4 : k & 1 ? (int)sizeof(XT) : (int)sizeof(HT);
-        if (P.t == 0) {
-            const char* p = static_cast<const char*>(arrays[k]) + (k == 4 ? 0 : (int64_t)c0 * size);
-            const int64_t step = strides[k] * size;
-            const int bytes = arrays[k] == nullptr ? 0 : k == 4 ? 16 : mine * size;
-            feeds[P.team][k] = {p + r0 * step, p, p + (d.rows - 1) * step + bytes, step, bytes, parts[k]};
-        }
-        there += arrays[k] != nullptr;
-        // An absent array's place holds zeros.
-        if (arrays[k] == nullptr)
-            for (int i = P.t; i < stages * (k & 1 ? xb : hb) / 4; i += G.threads) {
-                const int words = (k & 1 ? xb : hb) / 4;
-                reinterpret_cast<unsigned*>(stage0 + i / words * stage_bytes + parts[k])[i % words] = 0;
-            }
-    }
-    if (P.t == 0)
-        for (int k = 0; k < stages; ++k) bar_init(&full[P.team][k], there);
-    asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    constexpr int sizes[kFeeds] = {sizeof(HT), sizeof(XT), sizeof(HT), sizeof(XT), 4};
+    const int parts[kFeeds + 1] = {0, at_x, at_gn, at_gx, at_st, stage_bytes};
+    Ring<VECTOR> ring;
+    ring.stage0 = memory + (size_t)P.team * stages * stage_bytes;
+    ring.full = full[P.team];
+    ring.feeds = feeds[P.team];
+    ring.stages = stages;
+    ring.stage_bytes = stage_bytes;
+    ring.open(arrays, strides, sizes, parts, true, c0, mine, d.rows, r0, r1, P.t, G.threads);
     if (P.R.ctas > 1) cg::this_cluster().sync();
     else __syncthreads();
-
-    // The next row into the next stage, by the team's first warp.
-    const unsigned long long policy = read_once();
-    int left = (int)(r1 - r0), to = 0;   // rows to copy
-    const bool feeder = P.t < kFeeds && feeds[P.team][P.t < kFeeds ? P.t : 0].bytes > 0;
-    const auto copy_row = [&] {
-        if (left == 0) return;
-        if (feeder) feed_row<VECTOR>(feeds[P.team][P.t], stage0 + to * stage_bytes, &full[P.team][to], policy);
-        --left;
-        if (++to == stages) to = 0;
-    };
-    if (P.R.warp == 0)
-        for (int k = 0; k < stages - 1; ++k) copy_row();
+    ring.template start<kFeeds>(P.t);
 
     // Threads behind the row's end read its last values (VECTOR) or what lies
     // there, and drop them.
@@ -882,8 +1077,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     unsigned shifts[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const int size = k & 1 ? (int)sizeof(XT) : (int)sizeof(HT);
-        shifts[k] = VECTOR ? 0 : (unsigned)((uintptr_t)arrays[k] + (c0 + r0 * strides[k]) * size) & 15;
+        shifts[k] = VECTOR ? 0 : (unsigned)((uintptr_t)arrays[k] + (c0 + r0 * strides[k]) * sizes[k]) & 15;
     }
     F8 acc[kKinds], group[GROUPED ? 2 : 1], kp, kb, kw;
 #pragma unroll
@@ -895,9 +1089,6 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     HT* ho = static_cast<HT*>(g.grad_h) + r0 * d.dim;
     const float a = has_h ? d.residual_scale : 1.0f;
     int64_t turn = r0;   // the row at which another row of the gate begins
-    int stage = 0;
-    unsigned phase = 0;
-    bool lost = false;
     // The rows of every CTA of a cluster are the same, so all take part in its sums.
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, ho += d.dim) {
         const void* gate = d.gate;
@@ -908,13 +1099,9 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
             if (has_h) post_parameters<FULL>(d, gate, pb, cols, kp, kb);
             turn = GROUPED ? (r / per + 1) * per : r1;
         }
-        if (!lost && !bar_wait(&full[P.team][stage], phase)) {
-            lost = true;   // the results become NaN
-            if (P.t == 0) atomicAdd(&g_norm_timeouts, 1u);
-        }
-        const char* s0 = stage0 + stage * stage_bytes;
-        const float4 st = lost ? make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F)
-                               : *reinterpret_cast<const float4*>(s0 + at_st);
+        const char* s0 = ring.row(P.t);
+        const float4 st = ring.lost ? make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F)
+                                    : *reinterpret_cast<const float4*>(s0 + at_st);
         F8 hh, xh, dx, dn;
         const HT* gnr = reinterpret_cast<const HT*>(s0 + at_gn + shifts[2]);
         const XT* gxr = reinterpret_cast<const XT*>(s0 + at_gx + shifts[3]);
@@ -957,7 +1144,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
         P.R.template sum<kLog>(s);
         // Every thread is past the row before (a warp alone: in step): its stage is free.
         if (G.threads == 32) __syncwarp();
-        if (P.R.warp == 0) copy_row();
+        if (P.R.warp == 0) ring.copy_row(P.t);
         const float m1 = s[0] * inv;
         float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(st.w, s[2] - m1 * s[3], s[1]);
         if constexpr (FULL) {
@@ -1008,34 +1195,36 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
                 end_group<VECTOR, FULL>(g, gate, pb, cols, k0, edge, group, acc);
             }
         }
-        if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-        }
+        ring.next();
         if (!VECTOR)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                shifts[k] = (shifts[k] + (unsigned)strides[k] * (k & 1 ? sizeof(XT) : sizeof(HT))) & 15;
+                shifts[k] = (shifts[k] + (unsigned)strides[k] * sizes[k]) & 15;
     }
-    if (lost && P.t == 0)   // copies still on their way end before the CTA does
-        for (int64_t k = max((int64_t)0, r1 - r0 - stages); k < r1 - r0; ++k)
-            bar_wait(&full[P.team][k % stages], (unsigned)(k / stages) & 1);
+    ring.close(P.t, r1 - r0);
     __syncthreads();
-    end_sums<VECTOR, kKinds>(P, G, W, (int)d.dim, reinterpret_cast<float*>(ring), acc);
+    end_sums<VECTOR, kKinds>(P, G, W, (int)d.dim, reinterpret_cast<float*>(memory), acc);
     if (P.R.ctas > 1) cg::this_cluster().sync();
 }
 
-template <typename XT, typename HT, bool VECTOR>
+template <typename XT, typename HT>
 cudaError_t run_forward(const mdq_residual_norm_desc& d, const Teams& G, int chunks, int grid,
-                        int cluster, bool full, cudaStream_t stream) {
+                        int cluster, cudaStream_t stream) {
     typedef void (*Kernel)(const mdq_residual_norm_desc, const Teams);
-    const Kernel k = chunks == 1   ? (full ? (Kernel)norm_rows<XT, HT, VECTOR, 1, true>
-                                           : (Kernel)norm_rows<XT, HT, VECTOR, 1, false>)
-                     : chunks == 2 ? (full ? (Kernel)norm_rows<XT, HT, VECTOR, 2, true>
-                                           : (Kernel)norm_rows<XT, HT, VECTOR, 2, false>)
-                                   : (full ? (Kernel)norm_rows<XT, HT, VECTOR, 4, true>
-                                           : (Kernel)norm_rows<XT, HT, VECTOR, 4, false>);
+    const Kernel k = chunks == 1   ? (Kernel)norm_rows<XT, HT, 1>
+                     : chunks == 2 ? (Kernel)norm_rows<XT, HT, 2>
+                                   : (Kernel)norm_rows<XT, HT, 4>;
     return launch(k, dim3(grid), G.threads * G.teams, 0, stream, cluster, false, d, G);
+}
+
+template <typename XT, typename HT, bool VECTOR, bool FULL>
+cudaError_t run_ring(const mdq_residual_norm_desc& d, const Teams& G, int chunks, int grid, int cluster,
+                     int stages, size_t smem, cudaStream_t stream) {
+    typedef void (*Kernel)(const mdq_residual_norm_desc, const Teams, int);
+    const Kernel k = chunks == 1   ? (Kernel)norm_rows_ring<XT, HT, VECTOR, 1, FULL>
+                     : chunks == 2 ? (Kernel)norm_rows_ring<XT, HT, VECTOR, 2, FULL>
+                                   : (Kernel)norm_rows_ring<XT, HT, VECTOR, 4, FULL>;
+    return launch<215 * 1024>(k, dim3(grid), G.threads * G.teams, smem, stream, cluster, false, d, G, stages);
 }
 
 template <typename XT, typename HT, bool VECTOR>
@@ -1069,8 +1258,8 @@ cudaError_t run_backward(const mdq_residual_norm_grad_desc& g, const Teams& G, c
     DECL(float, float, ff) DECL(float, __nv_bfloat16, fb) DECL(__nv_bfloat16, __nv_bfloat16, bb)   \
         DECL(__nv_bfloat16, float, bf)
 #define MDQ_NORM_DECLARE(XT, HT, S)                                                                \
-    cudaError_t forward_##S(const mdq_residual_norm_desc&, const Teams&, int, int, int, bool,      \
-                            bool, cudaStream_t);                                                   \
+    cudaError_t forward_##S(const mdq_residual_norm_desc&, const Teams&, int, int, int, int,       \
+                            size_t, bool, bool, cudaStream_t);                                     \
     cudaError_t backward_##S(const mdq_residual_norm_grad_desc&, const Teams&, const Partials&,    \
                              int, int, int, bool, bool, bool, cudaStream_t);                       \
     cudaError_t stream_##S(const mdq_residual_norm_grad_desc&, const Teams&, const Partials&, int, \
@@ -1081,9 +1270,15 @@ MDQ_NORM_TYPES(MDQ_NORM_DECLARE)
 #define MDQ_NORM_INSTANTIATE(XT, HT, S)                                                            \
     namespace mdq_norm {                                                                           \
     cudaError_t forward_##S(const mdq_residual_norm_desc& d, const Teams& G, int chunks, int grid, \
-                            int cluster, bool vector, bool full, cudaStream_t stream) {            \
-        return vector ? run_forward<XT, HT, true>(d, G, chunks, grid, cluster, full, stream)       \
-                      : run_forward<XT, HT, false>(d, G, chunks, grid, cluster, full, stream);     \
+                            int cluster, int stages, size_t smem, bool vector, bool full,          \
+                            cudaStream_t stream) {                                                 \
+        if (stages == 0) return run_forward<XT, HT>(d, G, chunks, grid, cluster, stream);          \
+        return vector ? run_ring<XT, HT, true, true>(d, G, chunks, grid, cluster, stages, smem,    \
+                                                     stream)                                       \
+               : full ? run_ring<XT, HT, false, true>(d, G, chunks, grid, cluster, stages, smem,   \
+                                                      stream)                                      \
+                      : run_ring<XT, HT, false, false>(d, G, chunks, grid, cluster, stages, smem,  \
+                                                       stream);                                    \
     }                                                                                              \
     cudaError_t backward_##S(const mdq_residual_norm_grad_desc& g, const Teams& G,                 \
                              const Partials& W, int chunks, int grid, int cluster, bool vector,    \
