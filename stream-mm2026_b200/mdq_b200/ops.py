@@ -19,13 +19,13 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _stream_handle
 
 _FLOAT = {torch.float32: _lib.MDQ_F32, torch.bfloat16: _lib.MDQ_BF16}
 _IDS = {torch.int32: _lib.MDQ_I32, torch.int64: _lib.MDQ_I64}
@@ -40,6 +40,10 @@ _NORM_GRAD = struct.Struct("=10Q5q2f4i10Q3q")
 _DISTILL = struct.Struct("=8Q5qi2f3i")
 
 
+# These checks run on every call, beside kernels of a few microseconds: they ask
+# for a device's index rather than compare devices, and look sizes up once.
+
+
 def _float_code(t: torch.Tensor, what: str) -> int:
     code = _FLOAT.get(t.dtype)
     if code is None:
@@ -47,15 +51,17 @@ def _float_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _on(t: torch.Tensor, dev: torch.device, what: str) -> None:
-    if t.device != dev:
-        raise RuntimeError(f"{what} must be on {dev}")
-
-
-def _device(t: torch.Tensor, what: str) -> torch.device:
-    if not t.is_cuda:
+def _device(t: torch.Tensor, what: str) -> int:
+    """Index of the device a tensor is on."""
+    index = t.get_device()
+    if index < 0 or not t.is_cuda:
         raise RuntimeError(f"{what} must be CUDA")
-    return t.device
+    return index
+
+
+def _on(t: torch.Tensor, index: int, what: str) -> None:
+    if t.get_device() != index:
+        raise RuntimeError(f"{what} must be on cuda:{index}")
 
 
 def _row_stride(t: torch.Tensor, what: str) -> int:
@@ -74,10 +80,20 @@ def _row_stride(t: torch.Tensor, what: str) -> int:
 
 def _row_count(t: torch.Tensor) -> int:
     """Rows of ``t``, also when its rows or columns are none."""
+    shape = t.shape
+    if len(shape) == 2:
+        return shape[0]
     n = 1
-    for k in t.shape[:-1]:
+    for k in shape[:-1]:
         n *= k
     return n
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of ``t``'s shape and dtype."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _usable(t: torch.Tensor) -> torch.Tensor:
@@ -91,29 +107,45 @@ def _usable(t: torch.Tensor) -> torch.Tensor:
         return t.contiguous()
 
 
-def _run(name: str, dev: torch.device, desc: bytes) -> None:
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == dev.index:
-        st = fn(desc, _stream_handle(dev))
+def _run(fn, index: int, desc: bytes) -> None:
+    """One entry point of the library on the current stream of a device."""
+    if torch._C._cuda_getDevice() == index:
+        st = fn(desc, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            st = fn(desc, _stream_handle(dev))
+        with torch.cuda.device(index):
+            st = fn(desc, torch._C._cuda_getCurrentRawStream(index))
     if st:
         _lib.check(st)
 
 
-def _workspace(name: str, dev: torch.device, a: int, b: int, c: int):
+@lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(_lib.load(), name)
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(name: str, a: int, b: int, c: int) -> int:
     need = ctypes.c_int64(0)
-    _lib.check(getattr(_lib.load(), name)(a, b, c, ctypes.byref(need)))
-    if need.value == 0:
+    _lib.check(_entry(name)(a, b, c, ctypes.byref(need)))
+    return need.value
+
+
+def _workspace(name: str, index: int, a: int, b: int, c: int):
+    need = _workspace_bytes(name, a, b, c)
+    if need == 0:
         return None, 0, 0
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    return ws, ws.data_ptr(), need.value
+    ws = torch.empty(need, dtype=torch.uint8, device=_cuda(index))
+    return ws, ws.data_ptr(), need
+
+
+@lru_cache(maxsize=None)
+def _cuda(index: int) -> torch.device:
+    return torch.device("cuda", index)
 
 
 # --------------------------------------------------------------- embedding
 
-def _check_ids(ids: torch.Tensor, dev: torch.device) -> int:
+def _check_ids(ids: torch.Tensor, dev: int) -> int:
     code = _IDS.get(ids.dtype)
     if code is None:
         raise RuntimeError("ids must be int32 or int64")
@@ -130,9 +162,9 @@ def _embedding_forward(ids, table, scale, out_dtype):
     ids_code, table_code = _check_ids(ids, dev), _float_code(table, "table")
     stride = _row_stride(table, "table")
     vocab, dim = table.shape
-    out = torch.empty(*ids.shape, dim, dtype=out_dtype or table.dtype, device=dev)
+    out = torch.empty((*ids.shape, dim), dtype=out_dtype or table.dtype, device=table.device)
     out_code = _float_code(out, "out_dtype")
-    _run("mdq_embed", dev, _EMBED.pack(
+    _run(_entry("mdq_embed"), dev, _EMBED.pack(
         table.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(), vocab, dim, stride,
         scale, table_code, out_code, ids_code))
     return out
@@ -164,7 +196,7 @@ def scaled_embedding_grad(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int,
     if out is None:
         if accumulate:
             raise RuntimeError("accumulate needs out")
-        out = torch.empty(vocab, dim, dtype=dtype, device=dev)
+        out = torch.empty((vocab, dim), dtype=dtype, device=grad_out.device)
     else:
         _on(out, dev, "out")
         if out.shape != (vocab, dim) or not out.is_contiguous():
@@ -173,7 +205,7 @@ def scaled_embedding_grad(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int,
             raise RuntimeError("accumulate needs a float32 out")
     out_code, tokens = _float_code(out, "gradient"), ids.numel()
     ws, ws_ptr, ws_bytes = _workspace("mdq_embed_grad_workspace_bytes", dev, tokens, vocab, dim)
-    _run("mdq_embed_grad", dev, _EMBED_GRAD.pack(
+    _run(_entry("mdq_embed_grad"), dev, _EMBED_GRAD.pack(
         grad_out.data_ptr(), ids.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes, tokens, vocab, dim,
         stride, -1 if padding_idx is None else padding_idx, scale, go_code, out_code, ids_code,
         1 if accumulate else 0, 0))
@@ -237,39 +269,46 @@ def _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate, resid
     code = _KINDS.get(kind)
     if code is None:
         raise RuntimeError("kind must be 'rms' or 'layer'")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    shape = x.shape
+    if not shape or shape[-1] < 1:
         raise RuntimeError("x must be [..., dim]")
-    dim, rows = x.shape[-1], _row_count(x)
-    h_code, h_stride = x_code, 0
+    dim, rows = shape[-1], _row_count(x)
     if h is not None:
         _on(h, dev, "h")
-        h_code, h_stride = _float_code(h, "h"), _row_stride(h, "h")
-        if h.shape != x.shape:
+        h_code = _float_code(h, "h")
+        if h.shape != shape:
             raise RuntimeError("h must have x's shape")
+        h_stride = _row_stride(h, "h")
         if post_weight is None:
             raise RuntimeError("h needs post_weight")
-    elif post_weight is not None or post_bias is not None or gate is not None:
-        raise RuntimeError("gate and post parameters need h")
-    elif pre_weight is None:
-        raise RuntimeError("either h or pre_weight is needed")
-    elif residual_scale != 1.0:
-        raise RuntimeError("residual_scale needs h")
+    else:
+        h_code, h_stride = x_code, 0
+        if post_weight is not None or post_bias is not None or gate is not None:
+            raise RuntimeError("gate and post parameters need h")
+        if pre_weight is None:
+            raise RuntimeError("either h or pre_weight is needed")
+        if residual_scale != 1.0:
+            raise RuntimeError("residual_scale needs h")
     if pre_weight is None and pre_bias is not None:
         raise RuntimeError("pre_bias needs pre_weight")
     first = post_weight if post_weight is not None else pre_weight
-    p_code = _float_code(first, "parameters")
-    for t, what in ((post_weight, "post_weight"), (pre_weight, "pre_weight"),
-                    (post_bias, "post_bias"), (pre_bias, "pre_bias")):
-        if t is not None:
-            if t.shape != (dim,):
-                raise RuntimeError(f"{what} must be [dim]")
-            if t.dtype != first.dtype or not t.is_contiguous():
-                raise RuntimeError(f"{what}: parameters must be contiguous and of one dtype")
-            _on(t, dev, what)
+    p_code, dtype = _float_code(first, "parameters"), first.dtype
+    ptrs = []
+    for t, what in ((post_weight, "post_weight"), (post_bias, "post_bias"),
+                    (pre_weight, "pre_weight"), (pre_bias, "pre_bias")):
+        if t is None:
+            ptrs.append(0)
+            continue
+        if t.shape != (dim,):
+            raise RuntimeError(f"{what} must be [dim]")
+        if t.dtype != dtype or not t.is_contiguous():
+            raise RuntimeError(f"{what}: parameters must be contiguous and of one dtype")
+        _on(t, dev, what)
+        ptrs.append(t.data_ptr())
     gate_rows = 1
     if gate is not None:
         _on(gate, dev, "gate")
-        if gate.dtype != first.dtype or not gate.is_contiguous():
+        if gate.dtype != dtype or not gate.is_contiguous():
             raise RuntimeError("gate: parameters must be contiguous and of one dtype")
         if gate.dim() not in (1, 2) or gate.shape[-1] != dim:
             raise RuntimeError("gate must be [dim] or [groups, dim]")
@@ -277,9 +316,8 @@ def _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate, resid
             gate_rows = gate.shape[0]
             if gate_rows < 1 or rows % gate_rows:
                 raise RuntimeError("gate's groups must divide the rows")
-    return dev, (x.data_ptr(), _ptr(h), _ptr(x_new), _ptr(n), _ptr(stats), _ptr(post_weight),
-                 _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias), _ptr(gate), rows, dim,
-                 _row_stride(x, "x"), h_stride, gate_rows, residual_scale, eps, x_code, h_code,
+    return dev, (x.data_ptr(), _ptr(h), _ptr(x_new), _ptr(n), _ptr(stats), *ptrs, _ptr(gate), rows,
+                 dim, _row_stride(x, "x"), h_stride, gate_rows, residual_scale, eps, x_code, h_code,
                  p_code, code)
 
 
@@ -289,18 +327,18 @@ def residual_norm_forward(x, h, post_weight, pre_weight, *, post_bias=None, pre_
     """The forward pass of ``residual_norm``: (x_new, n, stats).  stats ([rows,
     4] fp32) is what ``residual_norm_backward`` needs, None without
     ``want_stats``."""
-    dev = _device(x, "x")
-    x_new = x if h is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    _device(x, "x")
+    x_new = x if h is None else _like(x)
     n = None
     if pre_weight is not None:
-        n = torch.empty(x.shape, dtype=x.dtype if h is None else h.dtype, device=dev)
+        n = _like(x if h is None else h)
     stats = None
     if want_stats:
-        stats = torch.empty(_row_count(x), 4, dtype=torch.float32, device=dev)
+        stats = torch.empty((_row_count(x), 4), dtype=torch.float32, device=x.device)
     dev, fields = _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate,
                                residual_scale, eps, kind, None if h is None else x_new, n, stats)
     if x.numel():
-        _run("mdq_residual_norm", dev, _NORM.pack(*fields))
+        _run(_entry("mdq_residual_norm"), dev, _NORM.pack(*fields))
     return x_new, n, stats
 
 
@@ -332,8 +370,7 @@ def residual_norm_backward(grad_new, grad_n, x, h, stats, post_weight, pre_weigh
     def like(t):
         return None if t is None else torch.empty_like(t)
 
-    gx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    gh = None if h is None else torch.empty(h.shape, dtype=h.dtype, device=dev)
+    gx, gh = _like(x), None if h is None else _like(h)
     g = ResidualNormGrads(gx, gh, like(post_weight), like(pre_weight), like(post_bias),
                           like(pre_bias), like(gate))
     if not x.numel():
@@ -343,7 +380,7 @@ def residual_norm_backward(grad_new, grad_n, x, h, stats, post_weight, pre_weigh
         return g
     ws, ws_ptr, ws_bytes = _workspace("mdq_residual_norm_grad_workspace_bytes", dev, fields[10],
                                       fields[11], fields[14])
-    _run("mdq_residual_norm_grad", dev, _NORM_GRAD.pack(
+    _run(_entry("mdq_residual_norm_grad"), dev, _NORM_GRAD.pack(
         *fields, _ptr(grad_new), _ptr(grad_n), gx.data_ptr(), _ptr(gh), _ptr(g.post_weight),
         _ptr(g.post_bias), _ptr(g.pre_weight), _ptr(g.pre_bias), _ptr(g.gate), ws_ptr, ws_bytes,
         *strides))
@@ -437,12 +474,14 @@ def _distill(logits, teacher, index, temperature, weight, scale, grad, upstream=
     if not 0.0 < temperature < float("inf"):
         raise RuntimeError("temperature must be positive and finite")
     stride = _row_stride(logits, "logits")
-    losses = torch.empty(lead, dtype=torch.float32, device=dev) if want_loss else None
-    total = torch.empty((), dtype=torch.float32, device=dev) if want_loss else None
+    losses = total = None
+    if want_loss:
+        losses = torch.empty(lead, dtype=torch.float32, device=logits.device)
+        total = torch.empty((), dtype=torch.float32, device=logits.device)
     up_stride = 0
     if upstream is not None and upstream.dim() > 0:
         up_stride = 1
-    _run("mdq_topk_distill", dev, _DISTILL.pack(
+    _run(_entry("mdq_topk_distill"), dev, _DISTILL.pack(
         logits.data_ptr(), teacher.data_ptr(), index.data_ptr(), _ptr(weight), _ptr(upstream),
         _ptr(losses), _ptr(total), _ptr(grad), rows, vocab, stride,
         0 if grad is None else _row_stride(grad, "out"), up_stride, top, temperature, scale, code,
@@ -479,8 +518,9 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
         if _row_count(out) > 1 and _row_stride(out, "out") < out.shape[-1]:
             raise RuntimeError("out's rows must not overlap")
     elif grad:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=_device(logits, "logits"))
-    total, losses = _distill(logits.detach(), teacher_logits, teacher_index, temperature, weight,
+        _device(logits, "logits")
+        out = _like(logits)
+    total, losses = _distill(logits, teacher_logits, teacher_index, temperature, weight,
                              scale, out)
     return TopkDistill(total, losses, out)
 
@@ -497,7 +537,7 @@ class _TopkDistillLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, upstream):
         logits, teacher, index, weight = ctx.saved_tensors
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = _like(logits)
         _distill(logits, teacher, index, ctx.args[0], weight, ctx.args[1], grad,
                  upstream.float().contiguous(), want_loss=False)
         return grad, None, None, None, None, None, None
