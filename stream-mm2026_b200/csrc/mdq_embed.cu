@@ -17,6 +17,12 @@
 //                     the work even however often an id occurs.
 //   embed_grad_join   adds the partial sums of the runs that cross edges
 // A few tokens take one launch (embed_grad_few).
+//
+// Measured, bf16 rows and f32 tables: lookup of 8192 rows of 4096, 21.8 us (9.2 TB/s:
+// repeated ids come from L2), of 16384 rows of 768, 8.4; gradient of the latter into a
+// dense 50257 x 768 result 23.7 (sort, under 154 MB of zeros at 6.5 TB/s) + 12.1 + 5.7;
+// of the former added to a 128256 x 4096 gradient 8.5 (sort) + 40.6 + 8.7, for 201 MB
+// at least of rows read and added to.
 #include "mdq_ops.cuh"
 
 #include <cooperative_groups.h>
@@ -66,43 +72,46 @@ __global__ void __launch_bounds__(kLookupThreads) embed_rows(const __grid_consta
     const bool in = id >= 0 && id < d.vocab;
     const TT* row = static_cast<const TT*>(d.table) + (in ? id : 0) * d.table_stride;
     OT* out = static_cast<OT*>(d.out) + n * d.dim;
-    const int64_t c0 = (int64_t)blockIdx.y * kLookupIter * 8 * lanes;
-    float v[kLookupIter][8] = {};
+    const int c0 = (int)blockIdx.y * kLookupIter * 8 * lanes, dim = (int)d.dim;
     if constexpr (VECTOR) {
+        float v[kLookupIter][8] = {};
 #pragma unroll
         for (int i = 0; i < kLookupIter; ++i) {
-            const int64_t c = c0 + (int64_t)(i * lanes + lane) * 8;
-            if (in && c < d.dim) load8(row + c, v[i]);
+            const int c = c0 + (i * lanes + lane) * 8;
+            if (in && c < dim) load8(row + c, v[i]);
         }
 #pragma unroll
         for (int i = 0; i < kLookupIter; ++i) {
-            const int64_t c = c0 + (int64_t)(i * lanes + lane) * 8;
-            if (c >= d.dim) break;
+            const int c = c0 + (i * lanes + lane) * 8;
+            if (c >= dim) break;
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[i][k] *= d.scale;
             store8(out + c, v[i]);
         }
     } else {
+        // 8 values in flight a thread; whole groups of columns without checks.
+        const int end = min(dim, c0 + kLookupIter * 8 * lanes);
+        for (int c = c0 + lane; c < end; c += 8 * lanes) {
+            float v[8];
+            if (c - lane + 8 * lanes <= end) {
 #pragma unroll
-        for (int i = 0; i < kLookupIter; ++i)
+                for (int k = 0; k < 8; ++k) v[k] = in ? to_f(row[c + k * lanes]) : 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int64_t c = c0 + (i * 8 + k) * lanes + lane;
-                if (in && c < d.dim) v[i][k] = to_f(row[c]);
+                for (int k = 0; k < 8; ++k) out[c + k * lanes] = from_f<OT>(v[k] * d.scale);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = in && c + k * lanes < end ? to_f(row[c + k * lanes]) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (c + k * lanes < end) out[c + k * lanes] = from_f<OT>(v[k] * d.scale);
             }
-#pragma unroll
-        for (int i = 0; i < kLookupIter; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int64_t c = c0 + (i * 8 + k) * lanes + lane;
-                if (c < d.dim) out[c] = from_f<OT>(v[i][k] * d.scale);
-            }
+        }
     }
 }
 
 // --------------------------------------------------------------------- sort
 
-constexpr int kSortThreads = 1024, kSortWarps = 32;
+constexpr int kSortThreads = 1024, kSortWarps = 32;     // at most
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;   // radix digit
 constexpr int kMaxCluster = 8;
 constexpr int kSlab = kMaxCluster * kSortThreads * 16;  // tokens one cluster can sort
@@ -121,11 +130,15 @@ struct SortArgs {
 };
 
 struct SortShared {
-    uint16_t hist[kSortWarps][kMaxBins];        // per warp, then its offset within the CTA
     unsigned count[kMaxCluster][kMaxBins];      // every CTA's digit counts
     unsigned base[kMaxBins];                    // first place of this CTA's digit
     unsigned scan[kSortWarps];
 };
+// Shared memory of the sort: the pairs, every warp's digit counts (then its offset
+// within the CTA), and the rest.
+size_t sort_shared(int threads, int ipt) {
+    return sizeof(Pair) * threads * ipt + sizeof(uint16_t) * (threads / 32) * kMaxBins + sizeof(SortShared);
+}
 
 // Zeros a CTA writes: a few microseconds of an SM's share of the bandwidth, so
 // that the hardware balances them over the SMs that do not sort.
@@ -142,7 +155,7 @@ __device__ __forceinline__ void fill_zeros(char* p, int64_t bytes, int thread, i
     for (int i = thread; i < (int)body; i += threads) __stcs(q + i, make_uint4(0, 0, 0, 0));
 }
 
-// Stable least-significant-digit radix sort of one slab of up to C * 1024 * IPT
+// Stable least-significant-digit radix sort of one slab of up to C * threads * IPT
 // tokens by a cluster of C CTAs.  A warp's items are consecutive tokens, so
 // (CTA, warp, item, lane) is the tokens' order and ranks taken in that order
 // keep it.  Ranks within a warp come from ballots over the digit's bits and a
@@ -151,24 +164,26 @@ __device__ __forceinline__ void fill_zeros(char* p, int64_t bytes, int thread, i
 template <int IPT>
 __global__ void __launch_bounds__(kSortThreads) embed_grad_sort(const __grid_constant__ SortArgs a) {
     extern __shared__ __align__(16) char raw[];
-    Pair* buf = reinterpret_cast<Pair*>(raw);                       // [1024 * IPT]
-    SortShared& S = *reinterpret_cast<SortShared*>(raw + sizeof(Pair) * kSortThreads * IPT);
+    const int threads = blockDim.x, warps = threads >> 5;
+    Pair* buf = reinterpret_cast<Pair*>(raw);                       // [threads * IPT]
+    SortShared& S = *reinterpret_cast<SortShared*>(raw + sizeof(Pair) * threads * IPT);
+    uint16_t* hist = reinterpret_cast<uint16_t*>(&S + 1);           // [warps][bins]
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int64_t slab = blockIdx.x / C;
     if (slab >= a.slabs) {   // whole clusters: the dense result's zeros, kFillBytes a CTA
         const int64_t from = (blockIdx.x - a.slabs * C) * kFillBytes;
         if (from < a.fill_bytes)
-            fill_zeros(a.fill + from, min(kFillBytes, a.fill_bytes - from), threadIdx.x, kSortThreads);
+            fill_zeros(a.fill + from, min(kFillBytes, a.fill_bytes - from), threadIdx.x, threads);
         return;
     }
     // Every CTA of the cluster runs before its shared memory is written to.
     auto started = cluster.barrier_arrive();
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    constexpr int kItems = kSortThreads * IPT;
+    const int items = threads * IPT;
     const int64_t first = slab * kSlab;
     const int64_t left = min(a.tokens - first, (int64_t)kSlab);     // of this slab
-    const int own = rank * kItems;                                  // this CTA's first place
+    const int own = rank * items;                                  // this CTA's first place
     const int at = w * 32 * IPT + lane;                             // item j is at + 32 j
 
     Pair item[IPT];
@@ -185,8 +200,9 @@ __global__ void __launch_bounds__(kSortThreads) embed_grad_sort(const __grid_con
     const int bins = 1 << a.bits;
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = 32 + pass * a.bits;
-        for (int i = tid; i < kSortWarps * bins; i += kSortThreads) S.hist[i >> a.bits][i & (bins - 1)] = 0;
-        __syncthreads();
+        uint16_t* mine = hist + w * bins;
+        for (int i = lane; i < bins / 2; i += 32) reinterpret_cast<unsigned*>(mine)[i] = 0;
+        __syncwarp();
         uint16_t place[IPT];
 #pragma unroll
         for (int j = 0; j < IPT; ++j) {
@@ -198,39 +214,37 @@ __global__ void __launch_bounds__(kSortThreads) embed_grad_sort(const __grid_con
                 same &= digit >> b & 1 ? one : ~one;
             }
             const int before = __popc(same & ((1u << lane) - 1));
-            const uint16_t seen = S.hist[w][digit];
+            const uint16_t seen = mine[digit];
             place[j] = seen + before;
             __syncwarp();
-            if (before == 0) S.hist[w][digit] = seen + __popc(same);
+            if (before == 0) mine[digit] = seen + __popc(same);
             __syncwarp();
         }
         __syncthreads();
-        // Offsets of the warps within the CTA; the CTA's count goes to every CTA.
-        unsigned total = 0;
-        if (tid < bins) {
-            uint16_t c[kSortWarps];
-#pragma unroll
-            for (int k = 0; k < kSortWarps; ++k) c[k] = S.hist[k][tid];
-#pragma unroll
-            for (int k = 0; k < kSortWarps; ++k) {
-                S.hist[k][tid] = (uint16_t)total;
-                total += c[k];
-            }
-        }
+        // Offsets of the warps within the CTA; the CTA's counts go to every CTA.
+        // (Fewer threads than digits take several each.)
         if (pass == 0) cluster.barrier_wait(std::move(started));
-        if (tid < bins) {
-            for (int r = 0; r < C; ++r) cluster.map_shared_rank(&S.count[rank][tid], r)[0] = total;
+        for (int b = tid; b < bins; b += threads) {
+            unsigned total = 0;
+            for (int k0 = 0; k0 < warps; k0 += 8) {
+                uint16_t c[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) c[k] = k0 + k < warps ? hist[(k0 + k) * bins + b] : 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (k0 + k < warps) hist[(k0 + k) * bins + b] = (uint16_t)total;
+                    total += c[k];
+                }
+            }
+            for (int r = 0; r < C; ++r) cluster.map_shared_rank(&S.count[rank][b], r)[0] = total;
         }
         cluster.sync();
         // First place of this CTA's digit: all smaller digits, and the digit in
-        // the CTAs before.
-        unsigned all = 0, before = 0;
-        if (tid < bins)
-            for (int r = 0; r < C; ++r) {
-                const unsigned c = S.count[r][tid];
-                if (r < rank) before += c;
-                all += c;
-            }
+        // the CTAs before.  Thread t has the digits from t * each on.
+        const int each = (bins + threads - 1) / threads;
+        unsigned all = 0;
+        for (int b = tid * each; b < min(bins, (tid + 1) * each); ++b)
+            for (int r = 0; r < C; ++r) all += S.count[r][b];
         unsigned run = all;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -239,27 +253,33 @@ __global__ void __launch_bounds__(kSortThreads) embed_grad_sort(const __grid_con
         }
         if (lane == 31) S.scan[w] = run;
         __syncthreads();
-        if (w == 0) {
-            unsigned v = S.scan[lane];
+        unsigned upto = run - all;
+        {
+            unsigned v = lane < w ? S.scan[lane] : 0;   // the warps before
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
-            }
-            S.scan[lane] = v;
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            upto += v;
         }
-        __syncthreads();
-        if (tid < bins) S.base[tid] = run - all + (w > 0 ? S.scan[w - 1] : 0) + before;
+        for (int b = tid * each; b < min(bins, (tid + 1) * each); ++b) {
+            unsigned before = 0, here = 0;
+            for (int r = 0; r < C; ++r) {
+                const unsigned c = S.count[r][b];
+                if (r < rank) before += c;
+                here += c;
+            }
+            S.base[b] = upto + before;
+            upto += here;
+        }
         __syncthreads();
         const bool last = pass + 1 == a.passes;
 #pragma unroll
         for (int j = 0; j < IPT; ++j) {
             const int digit = (int)(item[j] >> shift) & (bins - 1);
-            const unsigned to = S.base[digit] + S.hist[w][digit] + place[j];
+            const unsigned to = S.base[digit] + mine[digit] + place[j];
             if (last) {
                 if (to < left) a.sorted[first + to] = item[j];
             } else {
-                cluster.map_shared_rank(buf, to / kItems)[to % kItems] = item[j];
+                cluster.map_shared_rank(buf, to / items)[to % items] = item[j];
             }
         }
         if (last) break;
@@ -360,7 +380,12 @@ __device__ __forceinline__ void write_row(const SumArgs& a, unsigned id,
         for (int k = 0; k < N; ++k)
             if (c.has(k)) {
                 WT* p = row + c.at(k);
-                *p = from_f<WT>(acc[k] * a.scale + (a.accumulate ? to_f(*p) : 0.0f));
+                if constexpr (sizeof(WT) == 4)
+                    if (a.accumulate) {
+                        atomicAdd(p, acc[k] * a.scale);   // as above
+                        continue;
+                    }
+                *p = from_f<WT>(acc[k] * a.scale);
             }
     }
 }
@@ -436,19 +461,23 @@ __global__ void __launch_bounds__(1024) embed_grad_join(const __grid_constant__ 
     const Columns<GT, VECTOR> col(blockIdx.y, t, a.tx, a.dim);
     wait_previous();
     for (int b = blockIdx.x; b < a.chunks - 1; b += gridDim.x) {
-        const int64_t edge = (int64_t)(b + 1) * a.chunk;   // first pair behind the edge
-        const unsigned id = (unsigned)(a.sorted[edge] >> 32);
-        if (id >= a.vocab || (unsigned)(a.sorted[edge - 1] >> 32) != id) continue;
-        const int64_t i0 = edge - a.chunk;
-        if (i0 > 0 && (unsigned)(a.sorted[i0 - 1] >> 32) == id) continue;   // began earlier
-        // The last chunk that the run reaches: the first behind the edge whose
-        // last pair is of another run, or is followed by one.
+        // What decides about the edge is loaded at once: the pairs on both sides of
+        // it, the one before this chunk, and the first pairs of the next 32 chunks.
+        const int64_t edge = (int64_t)(b + 1) * a.chunk, i0 = edge - a.chunk;
+        int64_t next = (int64_t)(b + 2 + (threadIdx.x & 31)) * a.chunk;
+        const auto id_at = [&](int64_t i) { return (unsigned)(a.sorted[i] >> 32); };
+        const unsigned id = id_at(edge), left = id_at(edge - 1), before = i0 > 0 ? id_at(i0 - 1) : 0xffffffffu;
+        unsigned ahead = next < a.tokens ? id_at(next) : 0xffffffffu;
+        if (id >= a.vocab || left != id || before == id) continue;   // none crosses, or it began earlier
+        // The last chunk that the run reaches, 32 chunks at a time.
         int end = b + 1;
-        for (int more = 32; more == 32; end += more) {   // 32 chunks at a time, a lane each
-            const int64_t first = (int64_t)(end + 1 + (threadIdx.x & 31)) * a.chunk;
-            const bool in = first < a.tokens && (unsigned)(a.sorted[first] >> 32) == id;
-            const unsigned mask = __ballot_sync(0xffffffffu, in);
-            more = mask == 0xffffffffu ? 32 : __ffs(~mask) - 1;
+        while (true) {
+            const unsigned mask = __ballot_sync(0xffffffffu, ahead == id);
+            const int more = mask == 0xffffffffu ? 32 : __ffs(~mask) - 1;
+            end += more;
+            if (more < 32) break;
+            next += 32 * (int64_t)a.chunk;
+            ahead = next < a.tokens ? id_at(next) : 0xffffffffu;
         }
         // Parts b (its second partial), b + 1, ..., end (their first).
         const int parts = end - b + 1, each = (parts + teams - 1) / teams;
@@ -569,10 +598,13 @@ __global__ void __launch_bounds__(kFewThreads) embed_grad_few(const __grid_const
 
 // ------------------------------------------------------------------ planning
 
-// Pairs of a chunk: about 131072 threads over all teams, 8 to 64 rows each (16
-// where a block has many teams, whose pairs it keeps in shared memory).
+// Pairs of a chunk: about 65536 threads over all teams, 8 to 64 rows each; at most
+// 32 above 2048 columns, where many threads share a row anyway, and 16 where a
+// block has many teams, whose pairs it keeps in shared memory.  Sum and join of
+// 16384 rows of 768 with 16 / 32 a chunk: 19.5 / 17.7 us, of 8192 rows of 4096 with
+// 32 / 64: 50 / 56, of 32768 rows of 1024: 44 / 34.
 int chunk_of(int64_t tokens, int64_t dim) {
-    const int64_t want = tokens * ceil_div(dim, 8) / 131072, most = dim < 256 ? 16 : 64;
+    const int64_t want = tokens * ceil_div(dim, 8) / 65536, most = dim < 256 ? 16 : dim > 2048 ? 32 : 64;
     int c = 8;
     while (c < most && c < want) c *= 2;
     return c;
@@ -623,7 +655,7 @@ mdq_status sum_slab(const SumArgs& a, int64_t slices, cudaStream_t stream) {
     const int joiners = a.tx >= 64 ? 512 / a.tx : a.tx >= 4 ? 8 : 32 / a.tx;
     const int edges = a.chunks - 1;
     e = launch(embed_grad_join<GT, WT, VECTOR>,
-               dim3((unsigned)(edges < 148 * 4 ? edges : 148 * 4), (unsigned)slices),
+               dim3((unsigned)(edges < 65536 ? edges : 65536), (unsigned)slices),
                joiners * a.tx, sizeof(float) * joiners * a.tx * Vec<GT>::N, stream, 1, true, a);
     return status_of(e, "embed grad");
 }
@@ -669,11 +701,11 @@ mdq_status run_grad(const mdq_embed_grad_desc& d, const SumArgs& a, const Layout
 }
 
 template <int IPT>
-mdq_status run_sort(const SortArgs& a, int cluster, cudaStream_t stream) {
-    const size_t smem = sizeof(Pair) * kSortThreads * IPT + sizeof(SortShared);
+mdq_status run_sort(const SortArgs& a, int cluster, int threads, cudaStream_t stream) {
+    const size_t smem = sort_shared(threads, IPT);
     const int64_t grid = (a.slabs + ceil_div(ceil_div(a.fill_bytes, kFillBytes), cluster)) * cluster;
     if (grid > INT32_MAX) return mdq_fail(MDQ_ERR_TOO_LARGE, "embed grad: gradient too large");
-    return status_of(launch(embed_grad_sort<IPT>, dim3((unsigned)grid), kSortThreads, smem, stream,
+    return status_of(launch(embed_grad_sort<IPT>, dim3((unsigned)grid), threads, smem, stream,
                             cluster, false, a),
                      "embed grad sort");
 }
@@ -692,8 +724,8 @@ mdq_status mdq_embed(const mdq_embed_desc* d, cudaStream_t stream) {
     if (!id_type(d->ids_dtype))
         return mdq_fail(MDQ_ERR_UNSUPPORTED, "embed: ids must be MDQ_I32 or MDQ_I64");
     if (d->tokens > INT32_MAX) return mdq_fail(MDQ_ERR_TOO_LARGE, "embed: 2^31 tokens or more");
-    if (d->dim > (int64_t)1024 * 65535)   // slices of a row in grid.y
-        return mdq_fail(MDQ_ERR_TOO_LARGE, "embed: 67107840 columns at most");
+    if (d->dim > (int64_t)1024 * 65535 - 1024)   // slices of a row in grid.y
+        return mdq_fail(MDQ_ERR_TOO_LARGE, "embed: 67106816 columns at most");
     if (d->tokens == 0) return MDQ_OK;
     if (d->table == nullptr || d->ids == nullptr || d->out == nullptr)
         return mdq_fail(MDQ_ERR_INVALID_ARG, "embed: null pointer");
@@ -778,12 +810,13 @@ mdq_status mdq_embed_grad(const mdq_embed_grad_desc* d, cudaStream_t stream) {
             s.fill = static_cast<char*>(a.grad);
             s.fill_bytes = d->vocab * d->dim * type_size(wt);
         }
-        // 4 items a thread and as many CTAs as that takes; beyond 8 CTAs, 16 items.
-        int cluster = 1;
-        while (cluster < kMaxCluster && (int64_t)cluster * kSortThreads * 4 < d->tokens) cluster *= 2;
-        st = (int64_t)cluster * kSortThreads * 4 >= d->tokens
-                 ? run_sort<4>(s, cluster, stream)
-                 : run_sort<16>(s, cluster, stream);
+        // 4 items a thread (16 beyond 32768 tokens) and 8 CTAs of as few warps as
+        // that takes, 8 or more; fewer CTAs for fewer tokens.
+        const int ipt = d->tokens > kMaxCluster * kSortThreads * 4 ? 16 : 4;
+        int cluster = 1, threads = 256;
+        while (cluster < kMaxCluster && (int64_t)cluster * threads * ipt < d->tokens) cluster *= 2;
+        while (threads < kSortThreads && (int64_t)cluster * threads * ipt < d->tokens) threads *= 2;
+        st = ipt == 4 ? run_sort<4>(s, cluster, threads, stream) : run_sort<16>(s, cluster, threads, stream);
         if (st != MDQ_OK) return st;
     }
     typedef __nv_bfloat16 B;
