@@ -15,8 +15,9 @@
  * mdq_status from every entry point and mdq_last_error() for its reason.
  * Arguments are checked before anything is launched.  Sums, statistics and
  * exponentials are held in 32 bits or more; a result is rounded once, when it
- * is stored.  Results do not depend on the order in which blocks run: no
- * floating-point atomics.
+ * is stored.  Results do not depend on the order in which blocks run: sums are
+ * taken in fixed orders, and where an atomic addition joins a sum to a value in
+ * memory, it is the only one of its launch to that value.
  */
 #ifndef MDQ_OPS_H_
 #define MDQ_OPS_H_
@@ -145,7 +146,7 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* d, cudaStre
  *   c_n = scale * weight[n],  u_n = upstream[n * upstream_stride]
  * and loss = sum of row_loss.  An entry whose index lies outside [0, vocab) is
  * absent; a row of weight 0, or whose entries are all absent or -infinity, has
- * loss 0 and gradient 0 and its logits are not read.  Indices may repeat: each
+ * loss 0 and gradient 0 whatever its logits hold.  Indices may repeat: each
  * counts.  With top = 1 and temperature 1 this is the cross-entropy against
  * the index.
  */
@@ -160,7 +161,8 @@ typedef struct mdq_topk_distill_desc {
     float* row_loss;        /* [rows] or NULL                                      */
     float* loss;            /* [1] or NULL (needs row_loss)                        */
     void* grad;             /* [rows, vocab], logits_dtype, rows grad_stride apart,
-                               or NULL; may be `logits` itself                     */
+                               or NULL; may be `logits` itself (with its stride),
+                               else shares nothing with it                     */
     int64_t rows, vocab, logits_stride, grad_stride;
     int64_t upstream_stride;/* 0 (one value for all rows) or 1                     */
     int32_t top;            /* 1..MDQ_DISTILL_MAX_TOP                              */

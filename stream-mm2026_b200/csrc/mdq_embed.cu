@@ -512,11 +512,16 @@ __global__ void __launch_bounds__(1024) embed_grad_join(const __grid_constant__ 
     }
 }
 
-__global__ void __launch_bounds__(256) embed_grad_round(const float* from, __nv_bfloat16* to,
-                                                        int64_t n) {
+// The sums over several slabs into their result, or added to it (rows without a
+// token have sums of zero, and are not touched).
+template <typename WT, bool ADD>
+__global__ void __launch_bounds__(256) embed_grad_finish(const float* from, WT* to, int64_t n) {
     wait_previous();
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-        to[i] = __float2bfloat16_rn(from[i]);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const float v = from[i];
+        if constexpr (!ADD) to[i] = from_f<WT>(v);
+        else if (v != 0.0f) to[i] += v;
+    }
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -624,7 +629,8 @@ Layout layout_of(int64_t tokens, int64_t vocab, int64_t dim) {
     L.chunks = ceil_div(L.slab_tokens, L.chunk);
     L.partial_at = ceil_div(tokens * (int64_t)sizeof(Pair), 16) * 16;
     L.wide_at = L.partial_at + ceil_div(2 * L.chunks * dim * (int64_t)sizeof(float), 16) * 16;
-    // Several slabs are added in fp32 before a bf16 result is rounded.
+    // Several slabs are added in fp32 before a bf16 result is rounded, or before
+    // they are added to a gradient.
     L.bytes = L.wide_at + (L.slabs > 1 ? vocab * dim * (int64_t)sizeof(float) : 0);
     return L;
 }
@@ -683,7 +689,7 @@ mdq_status run_grad(const mdq_embed_grad_desc& d, SumArgs a, const Layout& L, cu
         a.tokens = (int32_t)(left < kSlab ? left : kSlab);
         a.chunk = (int32_t)L.chunk;
         a.chunks = (int32_t)ceil_div(a.tokens, L.chunk);
-        a.accumulate = d.accumulate || s > 0;
+        a.accumulate = a.accumulate || s > 0;
         const mdq_status st = sum_slab<GT, WT, VECTOR>(a, slices, stream);
         if (st != MDQ_OK) return st;
     }
@@ -781,7 +787,7 @@ mdq_status mdq_embed_grad(const mdq_embed_grad_desc* d, cudaStream_t stream) {
 
     const Layout L = layout_of(d->tokens, d->vocab, d->dim);
     char* ws = static_cast<char*>(d->workspace);
-    const bool wide = L.slabs > 1 && d->grad_dtype == MDQ_BF16;
+    const bool wide = L.slabs > 1 && (d->grad_dtype == MDQ_BF16 || d->accumulate);
     const int32_t wt = wide ? (int32_t)MDQ_F32 : d->grad_dtype;
     SumArgs a = {};
     a.grad_out = d->grad_out;
@@ -792,7 +798,7 @@ mdq_status mdq_embed_grad(const mdq_embed_grad_desc* d, cudaStream_t stream) {
     a.vocab = d->vocab;
     a.tokens = (int32_t)d->tokens;
     a.scale = d->scale;
-    a.accumulate = d->accumulate;
+    a.accumulate = d->accumulate && !wide;
     if (L.slabs > 0) {
         SortArgs s = {};
         s.ids = d->ids;
@@ -806,7 +812,7 @@ mdq_status mdq_embed_grad(const mdq_embed_grad_desc* d, cudaStream_t stream) {
         while (bits < 32 && (d->vocab >> bits) != 0) ++bits;   // ids up to vocab itself
         s.passes = (bits + kMaxBits - 1) / kMaxBits;
         s.bits = (bits + s.passes - 1) / s.passes;
-        if (!d->accumulate) {
+        if (!a.accumulate) {
             s.fill = static_cast<char*>(a.grad);
             s.fill_bytes = d->vocab * d->dim * type_size(wt);
         }
@@ -826,10 +832,14 @@ mdq_status mdq_embed_grad(const mdq_embed_grad_desc* d, cudaStream_t stream) {
         st = wt == MDQ_BF16 ? run_grad<float, B>(*d, a, L, stream)
                             : run_grad<float, float>(*d, a, L, stream);
     if (st != MDQ_OK || !wide) return st;
-    return status_of(launch(embed_grad_round, dim3(148 * 8), 256, 0, stream, 1, true,
-                            static_cast<const float*>(a.grad), static_cast<B*>(d->grad),
-                            d->vocab * d->dim),
-                     "embed grad");
+    const float* sums = static_cast<const float*>(a.grad);
+    const int64_t n = d->vocab * d->dim;
+    const dim3 grid(148 * 8);
+    const cudaError_t e =
+        d->accumulate
+            ? launch(embed_grad_finish<float, true>, grid, 256, 0, stream, 1, true, sums, static_cast<float*>(d->grad), n)
+            : launch(embed_grad_finish<B, false>, grid, 256, 0, stream, 1, true, sums, static_cast<B*>(d->grad), n);
+    return status_of(e, "embed grad");
 }
 
 }  // extern "C"

@@ -489,6 +489,22 @@ def _distill(logits, teacher, index, temperature, weight, scale, grad, upstream=
     return total, losses
 
 
+def _entangled(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [..., vocab] tensors of one shape and dtype share elements
+    without being the same: a row of one would be written before another reads it."""
+    rows, vocab, size = _row_count(a), a.shape[-1], a.element_size()
+    if rows == 0:
+        return False
+    off = b.data_ptr() - a.data_ptr()
+    sa, sb = ((_row_stride(t, "rows") if rows > 1 else 0) * size for t in (a, b))
+    if off >= (rows - 1) * sa + vocab * size or -off >= (rows - 1) * sb + vocab * size:
+        return False
+    if sa != sb:
+        return True
+    # the same distance between rows: side by side in one matrix, or the same rows
+    return off != 0 and (rows == 1 or not vocab * size <= off % sa <= sa - vocab * size)
+
+
 def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
                  *, temperature: float = 1.0, weight: Optional[torch.Tensor] = None,
                  scale: float = 1.0, grad: bool = True,
@@ -507,7 +523,7 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     hold.  top = 1 with temperature 1 is the cross-entropy against the index.
 
     ``out`` receives the gradient (logits' shape and dtype, evenly strided rows);
-    it may be ``logits``, which are then overwritten.  Without ``grad`` only the
+    it may be ``logits``, which are then overwritten, but share nothing else with them.  Without ``grad`` only the
     loss is computed."""
     if out is not None:
         if not grad:
@@ -517,6 +533,8 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
             raise RuntimeError("out must have logits' shape and dtype")
         if _row_count(out) > 1 and _row_stride(out, "out") < out.shape[-1]:
             raise RuntimeError("out's rows must not overlap")
+        if _entangled(logits, out):
+            raise RuntimeError("out must be logits itself or not overlap them")
     elif grad:
         _device(logits, "logits")
         out = _like(logits)
