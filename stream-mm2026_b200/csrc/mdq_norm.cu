@@ -483,12 +483,6 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
     if (g->f.rows > 0 && (g->f.stats == nullptr || g->grad_x == nullptr ||
                           (g->f.h != nullptr && g->grad_h == nullptr)))
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: null pointer");
-    int64_t need = 0;
-    st = mdq_residual_norm_grad_workspace_bytes(g->f.rows, g->f.dim, g->f.gate_rows, &need);
-    if (st != MDQ_OK) return st;
-    if (need > 0 && (g->workspace == nullptr || g->workspace_bytes < need))
-        return mdq_fail(MDQ_ERR_INVALID_ARG, "workspace holds %lld bytes, %lld needed",
-                        (long long)g->workspace_bytes, (long long)need);
     if (!aligned16(g->workspace) || !aligned16(g->f.stats))
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: workspace or stats misaligned");
     const bool grouped = g->f.gate_rows > 1;
@@ -498,8 +492,13 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
                      (g->grad_n == nullptr || rows16(g->grad_n, g->grad_n_stride, g->f.h_dtype));
     const int row_bytes = 2 * (int)(type_size(g->f.x_dtype) + type_size(g->f.h_dtype));
     GradPlan p;
-    if (!plan_stream(g->f.rows, g->f.dim, g->f.gate_rows, row_bytes, vec, full, &p) &&
-        !plan_grad(g->f.rows, g->f.dim, g->f.gate_rows, full, &p)) {
+    const bool planned = plan_stream(g->f.rows, g->f.dim, g->f.gate_rows, row_bytes, vec, full, &p) ||
+                         plan_grad(g->f.rows, g->f.dim, g->f.gate_rows, full, &p);
+    const int64_t need = planned ? p.bytes : g->f.rows * 2 * (int64_t)sizeof(float);
+    if (need > 0 && (g->workspace == nullptr || g->workspace_bytes < need))
+        return mdq_fail(MDQ_ERR_INVALID_ARG, "workspace holds %lld bytes, %lld needed",
+                        (long long)g->workspace_bytes, (long long)need);
+    if (!planned) {
         float* means = static_cast<float*>(g->workspace);
         if (g->f.rows > 0)
             norm_grad_wide<<<(unsigned)g->f.rows, kThreads, 0, stream>>>(*g, means);

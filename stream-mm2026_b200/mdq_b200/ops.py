@@ -107,6 +107,11 @@ def _usable(t: torch.Tensor) -> torch.Tensor:
         return t.contiguous()
 
 
+def _empty(shape, strides, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """torch.empty in two thirds of its host time (1.5 us against 2.3)."""
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+
+
 def _run(fn, index: int, desc: bytes) -> None:
     """One entry point of the library on the current stream of a device."""
     if torch._C._cuda_getDevice() == index:
@@ -134,7 +139,7 @@ def _workspace(name: str, index: int, a: int, b: int, c: int):
     need = _workspace_bytes(name, a, b, c)
     if need == 0:
         return None, 0, 0
-    ws = torch.empty(need, dtype=torch.uint8, device=_cuda(index))
+    ws = _empty((need,), (1,), torch.uint8, _cuda(index))
     return ws, ws.data_ptr(), need
 
 
@@ -196,7 +201,7 @@ def scaled_embedding_grad(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int,
     if out is None:
         if accumulate:
             raise RuntimeError("accumulate needs out")
-        out = torch.empty((vocab, dim), dtype=dtype, device=grad_out.device)
+        out = _empty((vocab, dim), (dim, 1), dtype, grad_out.device)
     else:
         _on(out, dev, "out")
         if out.shape != (vocab, dim) or not out.is_contiguous():
@@ -261,6 +266,16 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _parameter(t, shape, dtype, dev, what) -> int:
+    if t.shape != shape:
+        raise RuntimeError(f"{what} must be [dim]")
+    if t.dtype != dtype or not t.is_contiguous():
+        raise RuntimeError(f"{what}: parameters must be contiguous and of one dtype")
+    if t.get_device() != dev:
+        raise RuntimeError(f"{what} must be on cuda:{dev}")
+    return t.data_ptr()
+
+
 def _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate, residual_scale, eps,
                  kind, x_new, n, stats):
     """Checks the arguments and returns the fields of mdq_residual_norm_desc."""
@@ -291,20 +306,20 @@ def _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate, resid
             raise RuntimeError("residual_scale needs h")
     if pre_weight is None and pre_bias is not None:
         raise RuntimeError("pre_bias needs pre_weight")
-    first = post_weight if post_weight is not None else pre_weight
-    p_code, dtype = _float_code(first, "parameters"), first.dtype
-    ptrs = []
-    for t, what in ((post_weight, "post_weight"), (post_bias, "post_bias"),
-                    (pre_weight, "pre_weight"), (pre_bias, "pre_bias")):
-        if t is None:
-            ptrs.append(0)
-            continue
-        if t.shape != (dim,):
-            raise RuntimeError(f"{what} must be [dim]")
-        if t.dtype != dtype or not t.is_contiguous():
-            raise RuntimeError(f"{what}: parameters must be contiguous and of one dtype")
-        _on(t, dev, what)
-        ptrs.append(t.data_ptr())
+    first = pre_weight if post_weight is None else post_weight
+    dtype, one = first.dtype, (dim,)
+    p_code = _FLOAT.get(dtype)
+    if p_code is None:
+        raise RuntimeError("parameters must be float32 or bfloat16")
+    post_w = post_b = pre_w = pre_b = 0
+    if post_weight is not None:
+        post_w = _parameter(post_weight, one, dtype, dev, "post_weight")
+    if post_bias is not None:
+        post_b = _parameter(post_bias, one, dtype, dev, "post_bias")
+    if pre_weight is not None:
+        pre_w = _parameter(pre_weight, one, dtype, dev, "pre_weight")
+    if pre_bias is not None:
+        pre_b = _parameter(pre_bias, one, dtype, dev, "pre_bias")
     gate_rows = 1
     if gate is not None:
         _on(gate, dev, "gate")
@@ -316,8 +331,8 @@ def _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate, resid
             gate_rows = gate.shape[0]
             if gate_rows < 1 or rows % gate_rows:
                 raise RuntimeError("gate's groups must divide the rows")
-    return dev, (x.data_ptr(), _ptr(h), _ptr(x_new), _ptr(n), _ptr(stats), *ptrs, _ptr(gate), rows,
-                 dim, _row_stride(x, "x"), h_stride, gate_rows, residual_scale, eps, x_code, h_code,
+    return dev, (x.data_ptr(), _ptr(h), _ptr(x_new), _ptr(n), _ptr(stats), post_w, post_b, pre_w,
+                 pre_b, _ptr(gate), rows, dim, _row_stride(x, "x"), h_stride, gate_rows, residual_scale, eps, x_code, h_code,
                  p_code, code)
 
 
@@ -334,7 +349,7 @@ def residual_norm_forward(x, h, post_weight, pre_weight, *, post_bias=None, pre_
         n = _like(x if h is None else h)
     stats = None
     if want_stats:
-        stats = torch.empty((_row_count(x), 4), dtype=torch.float32, device=x.device)
+        stats = _empty((_row_count(x), 4), (4, 1), torch.float32, x.device)
     dev, fields = _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate,
                                residual_scale, eps, kind, None if h is None else x_new, n, stats)
     if x.numel():
@@ -367,12 +382,13 @@ def residual_norm_backward(grad_new, grad_n, x, h, stats, post_weight, pre_weigh
     if grad_n is not None and pre_weight is None:
         raise RuntimeError("grad_n needs pre_weight")
 
-    def like(t):
-        return None if t is None else torch.empty_like(t)
-
+    new = torch.empty_like
     gx, gh = _like(x), None if h is None else _like(h)
-    g = ResidualNormGrads(gx, gh, like(post_weight), like(pre_weight), like(post_bias),
-                          like(pre_bias), like(gate))
+    g = ResidualNormGrads(gx, gh, None if post_weight is None else new(post_weight),
+                          None if pre_weight is None else new(pre_weight),
+                          None if post_bias is None else new(post_bias),
+                          None if pre_bias is None else new(pre_bias),
+                          None if gate is None else new(gate))
     if not x.numel():
         for t in g:
             if t is not None:
@@ -476,8 +492,10 @@ def _distill(logits, teacher, index, temperature, weight, scale, grad, upstream=
     stride = _row_stride(logits, "logits")
     losses = total = None
     if want_loss:
-        losses = torch.empty(lead, dtype=torch.float32, device=logits.device)
-        total = torch.empty((), dtype=torch.float32, device=logits.device)
+        device = logits.device
+        losses = _empty(lead, (1,), torch.float32, device) if len(lead) == 1 else \
+            torch.empty(lead, dtype=torch.float32, device=device)
+        total = _empty((), (), torch.float32, device)
     up_stride = 0
     if upstream is not None and upstream.dim() > 0:
         up_stride = 1
