@@ -316,8 +316,12 @@ struct RowsPlan {
 // Forward: two chunks a thread for many rows above 256 columns, one for narrow
 // or few (as few threads as 512 allow), four where that is not enough.
 // 32768 bf16 rows of 768 / 128 columns: 48 / 18 us with two chunks, 108 / 15 with one.
-bool plan_forward(int64_t rows, int64_t dim, int64_t row_bytes, bool vec, bool ring, RowsPlan* p) {
-    for (int most = 4; most >= 1; most /= 2) {
+// Four chunks have their parameters loaded for every row, value by value off 16
+// bytes: rather twice the CTAs then (4112 bf16 rows of 16301: 284 against 488 us),
+// but for fp32 rows without means and biases (6704 of 10001: 400 against 296).
+bool plan_forward(int64_t rows, int64_t dim, int64_t row_bytes, bool vec, bool full, RowsPlan* p) {
+    const bool ring = full || !vec;
+    for (int most = vec || (row_bytes == 8 && !full) ? 4 : 2; most >= 1; most /= 2) {
         if (!plan_columns(dim, most, &p->cluster, &p->G)) return false;
         Teams& G = p->G;
         p->chunks = rows > 296 && G.share > 256 && most > 1 ? 2 : 1;
@@ -377,12 +381,13 @@ bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, bool full, GradPlan
     return true;
 }
 // With rows in a ring.  Above 8192 columns the steps between more than two CTAs
-// take longer than the other kernel's rows (503 against 382 us for 4096 rows of
-// 16384).
+// take longer than the other kernel's rows (437 against 385 us for 4096 bf16 rows of
+// 16384), but not than its loads of rows off 16 bytes (571 against 2549 us for 4112
+// rows of 16301).
 bool plan_stream(int64_t rows, int64_t dim, int64_t gate_rows, int64_t row_bytes, bool vec, bool full,
                  GradPlan* p) {
     p->chunks = 1;
-    if (!plan_columns(dim, 1, &p->cluster, &p->G) || p->cluster > 2) return false;
+    if (!plan_columns(dim, 1, &p->cluster, &p->G) || (vec && p->cluster > 2)) return false;
     Teams& G = p->G;
     G.threads = threads_for(G.share, 1);
     const int64_t stage = stage_of(row_bytes, 4, vec, G, 1) + 16;
@@ -444,7 +449,7 @@ mdq_status mdq_residual_norm(const mdq_residual_norm_desc* d, cudaStream_t strea
     RowsPlan p;
     const bool vec = vector_rows(a) && aligned16(a.x_new) && aligned16(a.n);
     const bool full = a.kind == MDQ_NORM_LAYER || a.post_bias != nullptr || a.pre_bias != nullptr;
-    if (plan_forward(a.rows, a.dim, type_size(a.x_dtype) + type_size(a.h_dtype), vec, full || !vec, &p))
+    if (plan_forward(a.rows, a.dim, type_size(a.x_dtype) + type_size(a.h_dtype), vec, full, &p))
         return status_of(MDQ_NORM_PICK(forward, a.x_dtype, a.h_dtype)(
                              a, p.G, p.chunks, p.grid, p.cluster, p.stages, p.smem, vec, full, stream),
                          "residual norm");
