@@ -35,12 +35,12 @@ struct Teams {
 };
 
 // The columns of one chunk of a thread: 8 consecutive ones on 16-byte boundaries
-// (VECTOR), or `step` apart.
+// (VECTOR), or 32 apart; a warp has 256 consecutive ones either way.
 template <bool VECTOR>
 struct Cols {
     int first, step, end;
-    __device__ __forceinline__ int at(int k) const { return first + (VECTOR ? k : k * step); }
-    __device__ __forceinline__ bool has(int k) const { return VECTOR ? first < end : at(k) < end; }
+    __device__ __forceinline__ int at(int k) const { return first + (VECTOR ? k : k * 32); }
+    __device__ __forceinline__ bool has(int k) const { return (VECTOR ? 0 : k * 32) < end - first; }
     // The thread's chunk i.
     __device__ __forceinline__ Cols chunk(int i) const { return {first + i * step * 8, step, end}; }
 };
@@ -112,11 +112,17 @@ struct Raw<T, false> {
 };
 
 template <typename T, bool VECTOR>
-__device__ __forceinline__ void store(T* row, const Cols<VECTOR>& c, const F8& v) {
+__device__ __forceinline__ void store(T* row, const Cols<VECTOR>& c, const F8& v, bool ragged = true) {
     if constexpr (!VECTOR) {
+        T* to = row + c.first;
+        if (!ragged) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) to[k * 32] = from_f<T>(value(v, k));
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (c.has(k)) row[c.at(k)] = from_f<T>(value(v, k));
+            if (c.has(k)) to[k * 32] = from_f<T>(value(v, k));
     } else if (c.has(0)) {
         if constexpr (sizeof(T) == 2) {
             *reinterpret_cast<uint4*>(row + c.first) =
@@ -184,9 +190,9 @@ __device__ __forceinline__ void post_parameters(const mdq_residual_norm_desc& d,
 }
 // The values less `mean` inside of the row; outside they are 0 and stay 0.
 template <bool VECTOR>
-__device__ __forceinline__ void less(F8& v, const Cols<VECTOR>& c, float mean) {
-    if constexpr (VECTOR) {
-        const float2 m = both(c.has(0) ? -mean : 0.0f);
+__device__ __forceinline__ void less(F8& v, const Cols<VECTOR>& c, float mean, bool ragged) {
+    if (VECTOR || !ragged) {
+        const float2 m = both(!ragged || c.has(0) ? -mean : 0.0f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = add(v[j], m);
     } else {
@@ -276,7 +282,7 @@ struct Place {
         R.parity = 0;
         const int c0 = R.rank * G.share;
         cols.end = min(dim, c0 + G.share);
-        cols.first = c0 + (VECTOR ? 8 * t : t);
+        cols.first = c0 + (VECTOR ? 8 * t : 8 * (t & ~31) + (t & 31));
         cols.step = G.threads;
         index = (int64_t)(blockIdx.x / R.ctas) * G.teams + team;
         count = (int64_t)(gridDim.x / R.ctas) * G.teams;
@@ -292,10 +298,10 @@ static __device__ unsigned int g_norm_timeouts;
 
 // A chunk's eight values in shared memory, the row's first at `row`.
 template <typename T, bool VECTOR>
-__device__ __forceinline__ void from_shared(const T* row, int at, int step, F8& v) {
+__device__ __forceinline__ void from_shared(const T* row, int at, F8& v) {
     if constexpr (!VECTOR) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) set(v, k, to_f(row[at + k * step]));
+        for (int k = 0; k < 8; ++k) set(v, k, to_f(row[at + k * 32]));
     } else if constexpr (sizeof(T) == 2) {
         unpack(*reinterpret_cast<const uint4*>(row + at), v);
     } else {
@@ -438,7 +444,7 @@ struct Ring {
 // their mean.
 template <int I, bool VECTOR>
 __device__ __forceinline__ float2 statistics(Reducer& R, const Cols<VECTOR>& cols, F8 (&v)[I],
-                                             bool layer, float inv, float eps) {
+                                             bool layer, bool ragged, float inv, float eps) {
     float mean = 0.0f;
     if (layer) {
         float2 t = both(0.0f);
@@ -450,7 +456,7 @@ __device__ __forceinline__ float2 statistics(Reducer& R, const Cols<VECTOR>& col
         R.sum<0>(s);
         mean = s[0] * inv;
 #pragma unroll
-        for (int i = 0; i < I; ++i) less(v[i], cols.chunk(i), mean);
+        for (int i = 0; i < I; ++i) less(v[i], cols.chunk(i), mean, ragged);
     }
     float2 t = both(0.0f);
 #pragma unroll
@@ -525,7 +531,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
         }
         if (kKeep && r + 1 < r1) fetch();
         if (h != nullptr) {
-            st.y = statistics<I>(P.R, cols, v, false, inv, d.eps).y;
+            st.y = statistics<I>(P.R, cols, v, false, false, inv, d.eps).y;
 #pragma unroll
             for (int i = 0; i < I; ++i) {
                 const Cols<true> c = cols.chunk(i);
@@ -547,7 +553,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
             for (int i = 0; i < I; ++i) rx[i].get(v[i]);
         }
         if (d.n != nullptr) {
-            st.w = statistics<I>(P.R, cols, v, false, inv, d.eps).y;
+            st.w = statistics<I>(P.R, cols, v, false, false, inv, d.eps).y;
 #pragma unroll
             for (int i = 0; i < I; ++i) {
                 const Cols<true> c = cols.chunk(i);
@@ -615,8 +621,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
         }
     }
     // Threads behind the row's end read its last values (VECTOR) or what lies
-    // there, and drop them.
-    const bool ragged = lanes != mine;
+    // there, and drop them (in warps that reach there: `ragged`).
+    const bool ragged = ((I - 1) * G.threads + P.R.warp * 32 + 32) * 8 > mine;
     const auto place = [&](int i) {
         const int at = cols.chunk(i).first - c0;
         return VECTOR ? min(at, mine - 8) : at;
@@ -654,10 +660,10 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
         if (has_h) {
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                from_shared<HT, VECTOR>(hr, place(i), cols.step, v[i]);
+                from_shared<HT, VECTOR>(hr, place(i), v[i]);
                 if (ragged) within_row(v[i], cols.chunk(i));
             }
-            float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
+            float2 s = statistics<I>(P.R, cols, v, layer, ragged, inv, d.eps);
             refill();
             if (ring.lost) s.y = CUDART_NAN_F;
             st.x = s.x;
@@ -675,7 +681,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
                 } else {
                     post_parameters<FULL>(d, gate, pb, c, p, b);
                 }
-                from_shared<XT, VECTOR>(xr, place(i), cols.step, xv);
+                from_shared<XT, VECTOR>(xr, place(i), xv);
                 if (ragged) within_row(xv, c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -684,17 +690,17 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
                     else v[i][j] = mul(v[i][j], p[j]);
                     v[i][j] = fma(both(d.residual_scale), xv[j], v[i][j]);
                 }
-                store(xo, c, v[i]);
+                store(xo, c, v[i], ragged);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                from_shared<XT, VECTOR>(xr, place(i), cols.step, v[i]);
+                from_shared<XT, VECTOR>(xr, place(i), v[i]);
                 if (ragged) within_row(v[i], cols.chunk(i));
             }
         }
         if (d.n != nullptr) {
-            float2 s = statistics<I>(P.R, cols, v, layer, inv, d.eps);
+            float2 s = statistics<I>(P.R, cols, v, layer, ragged, inv, d.eps);
             if (!has_h) refill();
             if (ring.lost) s.y = CUDART_NAN_F;
             st.z = s.x;
@@ -719,7 +725,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
                     if (FULL) v[i][j] = fma(v[i][j], w[j], b[j]);
                     else v[i][j] = mul(v[i][j], w[j]);
                 }
-                store(no, c, v[i]);
+                store(no, c, v[i], ragged);
             }
         }
         if (d.stats != nullptr && P.t == 0 && P.R.rank == 0)
@@ -1070,8 +1076,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     ring.template start<kFeeds>(P.t);
 
     // Threads behind the row's end read its last values (VECTOR) or what lies
-    // there, and drop them.
-    const bool ragged = lanes != mine;
+    // there, and drop them (in warps that reach there: `ragged`).
+    const bool ragged = (P.R.warp + 1) * 256 > mine;
     const int at = VECTOR ? min(cols.first - c0, mine - 8) : cols.first - c0;
     // Bytes by which the arrays' rows start behind a 16-byte boundary.
     unsigned shifts[4];
@@ -1105,10 +1111,10 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
         F8 hh, xh, dx, dn;
         const HT* gnr = reinterpret_cast<const HT*>(s0 + at_gn + shifts[2]);
         const XT* gxr = reinterpret_cast<const XT*>(s0 + at_gx + shifts[3]);
-        from_shared<XT, VECTOR>(reinterpret_cast<const XT*>(s0 + at_x + shifts[1]), at, cols.step, xh);
-        from_shared<HT, VECTOR>(gnr, at, cols.step, dn);
-        from_shared<XT, VECTOR>(gxr, at, cols.step, dx);
-        from_shared<HT, VECTOR>(reinterpret_cast<const HT*>(s0 + shifts[0]), at, cols.step, hh);
+        from_shared<XT, VECTOR>(reinterpret_cast<const XT*>(s0 + at_x + shifts[1]), at, xh);
+        from_shared<HT, VECTOR>(gnr, at, dn);
+        from_shared<XT, VECTOR>(gxr, at, dx);
+        from_shared<HT, VECTOR>(reinterpret_cast<const HT*>(s0 + shifts[0]), at, hh);
         if (ragged) {
             within_row(xh, cols);
             within_row(dn, cols);
@@ -1158,8 +1164,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
         const float rx = has_gn ? st.w : 0.0f;
         F8 o;
         if (FULL) {   // read again: the registers were the sums'
-            from_shared<HT, VECTOR>(gnr, at, cols.step, dn);
-            from_shared<XT, VECTOR>(gxr, at, cols.step, dx);
+            from_shared<HT, VECTOR>(gnr, at, dn);
+            from_shared<XT, VECTOR>(gxr, at, dx);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1170,7 +1176,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
             if (FULL) acc[FULL ? kPreBias : 0][j] = add(acc[FULL ? kPreBias : 0][j], dn[j]);
             o[j] = mul(both(a), dx[j]);
         }
-        store(xo, cols, o);
+        store(xo, cols, o, ragged);
         if (has_h) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1185,7 +1191,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
                     if (FULL) acc[FULL ? kPostBias : 0][j] = add(acc[FULL ? kPostBias : 0][j], dx[j]);
                 }
             }
-            store(ho, cols, o);
+            store(ho, cols, o, ragged);
         }
         if constexpr (GROUPED) {
             if (r + 1 == r1 || r + 1 == turn) {   // the group ends, or this team's part of it
