@@ -241,3 +241,65 @@ def test_operators_in_a_captured_graph(cuda_device):
     torch.cuda.synchronize()
     for a, b in zip(held, step()):
         assert torch.equal(a, b)
+
+
+def test_embedding_long_activations(cuda_device):
+    """Activations and incoming gradients of more than 2^31 elements."""
+    tokens, vocab, dim = 70000, 64, 32768
+    g = gen(61)
+    table = randn(g, vocab, dim, dtype=BF16).to(cuda_device)
+    ids = torch.randint(0, vocab - 1, (tokens,), generator=g).to(cuda_device)
+    ids[-1] = vocab - 1
+    out = ops.scaled_embedding(ids, table, 1.0)
+    for n in (0, 65535, 65536, tokens - 2, tokens - 1):
+        assert torch.equal(out[n], table[ids[n]])
+    out[:-1] = 0
+    grad = ops.scaled_embedding_grad(ids, out, vocab, 2.0)
+    assert torch.equal(grad[-1], table[-1].float() * 2) and not bool(grad[:-1].any())
+
+
+def test_residual_norm_long_activations(cuda_device):
+    """Rows whose element offsets pass 2^31: the last rows against the same rows
+    alone, and the parameters' gradients when only they have an upstream one."""
+    rows, dim, last = 66000, 32768, 3
+    g = gen(62)
+    w1, w2, gate = ((1 + randn(g, dim, scale=0.1)).to(cuda_device) for _ in range(3))
+    x = torch.zeros(rows, dim, dtype=BF16, device=cuda_device)
+    h = torch.zeros(rows, dim, dtype=BF16, device=cuda_device)
+    up = torch.zeros(rows, dim, dtype=BF16, device=cuda_device)
+    parts = [randn(g, last, dim, dtype=BF16).to(cuda_device) for _ in range(3)]
+    for t, p in zip((x, h, up), parts):
+        t[-last:] = p
+    new, n, stats = ops.residual_norm_forward(x, h, w1, w2, gate=gate)
+    b = ops.residual_norm_backward(up, up, x, h, stats, w1, w2, gate=gate)
+    leaves = [d64(t).requires_grad_() for t in (*parts[:2], w1, w2, gate)]
+    want = ref.residual_norm(leaves[0], leaves[1], leaves[2], leaves[3], gate=leaves[4])
+    grads = torch.autograd.grad(want, leaves, [d64(parts[2])] * 2)
+    u16 = rounding(BF16)
+    for got, w in zip((new, n), want):
+        w = w.detach()
+        within(got[-last:], w, u16 * w.abs() + 64 * U32 * 16)
+        assert not bool(got[:-last].any())
+    for got, w in zip((b.x[-last:], b.h[-last:], b.post_weight, b.pre_weight, b.gate), grads):
+        # sums over a row of 32768: 256 u of terms below 16, as many as sqrt(32768) of one sign
+        within(got, w, rounding(got.dtype) * w.abs() + 256 * U32 * 16 * 12)
+    assert not bool(b.x[:-last].any())
+
+
+def test_distill_indices_beyond_32_bits(cuda_device):
+    g = gen(63)
+    z, t = randn(g, 5, 300), randn(g, 5, 4)
+    idx = torch.randint(0, 300, (5, 4), generator=g)
+    idx[0, 1], idx[1, 2], idx[2, 0] = 1 << 32, (1 << 40) + 7, -(1 << 33)
+    idx[3] = torch.tensor([1 << 31, (1 << 32) + 1, -1, 1 << 62])
+    got = base._check_distill(cuda_device, z, t, idx, 1.0, None, 1.0)
+    assert float(got.rows[3]) == 0.0
+    ids = torch.tensor([1, 1 << 32, (1 << 33) + 1, -(1 << 40), 2], device=cuda_device)
+    table = randn(g, 4, 24).to(cuda_device)
+    out = ops.scaled_embedding(ids, table)
+    assert torch.equal(out[[0, 4]], table[[1, 2]]) and not bool(out[1:4].any())
+    grad = ops.scaled_embedding_grad(ids, out + 1, 4)
+    assert torch.equal(grad[[1, 2]], table[[1, 2]] + 1) and not bool(grad[[0, 3]].any())
+    long = ids.repeat(300)
+    grad = ops.scaled_embedding_grad(long, torch.ones(1500, 24, device=cuda_device), 4)
+    assert torch.equal(grad[:, 0].cpu(), torch.tensor([0.0, 300.0, 300.0, 0.0]))
