@@ -809,8 +809,9 @@ __device__ __forceinline__ void end_sums(const Place<VECTOR>& P, const Teams& G,
     }
 }
 
-// With q = g w1 hh and p = g w1, the gradient u = t p of the normalised block has
-//   sum u hh = sum dx q + r2 (sum e q - m0 sum q - m1 sum xh q)
+// With q = g w1 hh, p = g w1 and f = dx + r2 e, the gradient u = t p of the
+// normalised block has
+//   sum u hh = sum f q - r2 (m0 sum q + m1 sum xh q)
 // (and sum u the same with p for q), so that all sums of a row are taken in one
 // step, from which m1 = mean(e xh), m0 = mean(e) and the means of u follow.
 //
@@ -826,7 +827,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
                                                            mdq_residual_norm_grad_desc g,
                                                            const __grid_constant__ Teams G,
                                                            const __grid_constant__ Partials W) {
-    constexpr int kLog = FULL ? 4 : 2, kKinds = FULL ? 4 : 2;
+    constexpr int kLog = FULL ? 3 : 2, kKinds = FULL ? 4 : 2;
     __shared__ float slots[2 * kSlots * (1 << kLog)];
     extern __shared__ __align__(16) float shared[];   // [kinds][share]
     const mdq_residual_norm_desc& d = g.f;
@@ -921,9 +922,10 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
             }
         };
         F8 hh, xh, e, p;
-        float2 s2[FULL ? 10 : 4];
+        const float rx = gn != nullptr ? st.w : 0.0f, a = h != nullptr ? d.residual_scale : 1.0f;
+        float2 s2[FULL ? 8 : 3];
 #pragma unroll
-        for (int j = 0; j < (FULL ? 10 : 4); ++j) s2[j] = both(0.0f);
+        for (int j = 0; j < (FULL ? 8 : 3); ++j) s2[j] = both(0.0f);
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             F8 dx;
@@ -932,35 +934,33 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float2 q = mul(p[j], hh[j]);
+                const float2 f = fma(both(rx), e[j], dx[j]);
                 s2[0] = fma(e[j], xh[j], s2[0]);
-                s2[1] = fma(dx[j], q, s2[1]);
-                s2[2] = fma(e[j], q, s2[2]);
-                s2[3] = fma(xh[j], q, s2[3]);
+                s2[1] = fma(f, q, s2[1]);
+                s2[2] = fma(xh[j], q, s2[2]);
                 if constexpr (FULL) {
-                    s2[4] = add(s2[4], e[j]);
-                    s2[5] = add(s2[5], q);
-                    s2[6] = fma(dx[j], p[j], s2[6]);
-                    s2[7] = fma(e[j], p[j], s2[7]);
-                    s2[8] = fma(xh[j], p[j], s2[8]);
-                    s2[9] = add(s2[9], p[j]);
+                    s2[3] = add(s2[3], e[j]);
+                    s2[4] = add(s2[4], q);
+                    s2[5] = fma(f, p[j], s2[5]);
+                    s2[6] = fma(xh[j], p[j], s2[6]);
+                    s2[7] = add(s2[7], p[j]);
                 }
             }
         }
         float s[1 << kLog] = {};
 #pragma unroll
-        for (int j = 0; j < (FULL ? 10 : 4); ++j) s[j] = s2[j].x + s2[j].y;
+        for (int j = 0; j < (FULL ? 8 : 3); ++j) s[j] = s2[j].x + s2[j].y;
         P.R.template sum<kLog>(s);
         const float m1 = s[0] * inv;
-        float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(st.w, s[2] - m1 * s[3], s[1]);
+        float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(-rx * m1, s[2], s[1]);
         if constexpr (FULL) {
             if (layer) {
-                m0 = s[4] * inv;
-                u1 = fmaf(st.w, s[2] - m0 * s[5] - m1 * s[3], s[1]);
-                u0 = fmaf(st.w, s[7] - m0 * s[9] - m1 * s[8], s[6]) * inv;
+                m0 = s[3] * inv;
+                u1 = fmaf(-rx * m0, s[4], u1);
+                u0 = fmaf(-rx * m0, s[7], fmaf(-rx * m1, s[6], s[5])) * inv;
             }
         }
         u1 *= inv;
-        const float rx = gn != nullptr ? st.w : 0.0f, a = h != nullptr ? d.residual_scale : 1.0f;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             const Cols<VECTOR> c = cols.chunk(i);
@@ -1042,7 +1042,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
                                                              const __grid_constant__ Teams G,
                                                              const __grid_constant__ Partials W,
                                                              int stages) {
-    constexpr int kLog = FULL ? 4 : 2, kKinds = FULL ? 4 : 2;
+    constexpr int kLog = FULL ? 3 : 2, kKinds = FULL ? 4 : 2;
     __shared__ float slots[2 * kSlots * (1 << kLog)];
     __shared__ unsigned long long full[kTeam / 32][kMaxStages];
     __shared__ Feed feeds[kTeam / 32][kFeeds];
@@ -1121,7 +1121,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
             within_row(dx, cols);
             within_row(hh, cols);
         }
-        float2 s2[FULL ? 10 : 4];
+        const float rx = has_gn ? st.w : 0.0f;
+        float2 s2[FULL ? 8 : 3];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (FULL) hh[j] = add(hh[j], both(-st.x));
@@ -1131,37 +1132,35 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
             else xh[j] = fma(both(a), xh[j], q);
             xh[j] = mul(xh[j], both(st.w));
             const auto take = [&](int i, float2 x, float2 y) { s2[i] = j == 0 ? mul(x, y) : fma(x, y, s2[i]); };
+            const float2 f = fma(both(rx), e, dx[j]);
             take(0, e, xh[j]);
-            take(1, dx[j], q);
-            take(2, e, q);
-            take(3, xh[j], q);
+            take(1, f, q);
+            take(2, xh[j], q);
             if constexpr (FULL) {
-                s2[4] = j == 0 ? e : add(s2[4], e);
-                s2[5] = j == 0 ? q : add(s2[5], q);
-                take(6, dx[j], kp[j]);
-                take(7, e, kp[j]);
-                take(8, xh[j], kp[j]);
-                s2[9] = j == 0 ? kp[j] : add(s2[9], kp[j]);
+                s2[3] = j == 0 ? e : add(s2[3], e);
+                s2[4] = j == 0 ? q : add(s2[4], q);
+                take(5, f, kp[j]);
+                take(6, xh[j], kp[j]);
+                s2[7] = j == 0 ? kp[j] : add(s2[7], kp[j]);
             }
         }
         float s[1 << kLog] = {};
 #pragma unroll
-        for (int j = 0; j < (FULL ? 10 : 4); ++j) s[j] = s2[j].x + s2[j].y;
+        for (int j = 0; j < (FULL ? 8 : 3); ++j) s[j] = s2[j].x + s2[j].y;
         P.R.template sum<kLog>(s);
         // Every thread is past the row before (a warp alone: in step): its stage is free.
         if (G.threads == 32) __syncwarp();
         if (P.R.warp == 0) ring.copy_row(P.t);
         const float m1 = s[0] * inv;
-        float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(st.w, s[2] - m1 * s[3], s[1]);
+        float m0 = 0.0f, u0 = 0.0f, u1 = fmaf(-rx * m1, s[2], s[1]);
         if constexpr (FULL) {
             if (layer) {
-                m0 = s[4] * inv;
-                u1 = fmaf(st.w, s[2] - m0 * s[5] - m1 * s[3], s[1]);
-                u0 = fmaf(st.w, s[7] - m0 * s[9] - m1 * s[8], s[6]) * inv;
+                m0 = s[3] * inv;
+                u1 = fmaf(-rx * m0, s[4], u1);
+                u0 = fmaf(-rx * m0, s[7], fmaf(-rx * m1, s[6], s[5])) * inv;
             }
         }
         u1 *= inv;
-        const float rx = has_gn ? st.w : 0.0f;
         F8 o;
         if (FULL) {   // read again: the registers were the sums'
             from_shared<HT, VECTOR>(gnr, at, dn);
