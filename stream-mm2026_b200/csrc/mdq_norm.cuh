@@ -230,6 +230,19 @@ struct Reducer {
         float r = v[0];   // of value lane / kGroup
 #pragma unroll
         for (int o = kGroup / 2; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+        if (LOG == 0 && ctas == 1) {
+            if (warps > 1) {   // 16 at most, in both halves of a warp
+                float* buf = slots + parity * size + base;
+                parity ^= 1;
+                if (lane == 0) buf[warp] = r;
+                asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(warps * 32) : "memory");
+                r = (lane & 15) < warps ? buf[lane & 15] : 0.0f;
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+            }
+            v[0] = r;
+            return;
+        }
         if (warps > 1 || ctas > 1) {
             float* buf = slots + parity * size + base * NV;
             parity ^= 1;   // the other buffer is read until every thread is past the next barrier
@@ -267,17 +280,19 @@ struct Place {
     int t, team;
     int64_t index, count;   // of the team among all
     __device__ __forceinline__ Place(const Teams& G, int dim, float* slots, int size) {
-        team = threadIdx.x / G.threads;
-        t = threadIdx.x - team * G.threads;
+        // From the warp's first lane: the compiler then knows that a warp is in one team.
+        const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), warps = G.threads >> 5;
+        team = warp / warps;
+        t = (int)threadIdx.x - team * G.threads;
         cg::cluster_group cluster = cg::this_cluster();
         R.ctas = (int)cluster.num_blocks();
         R.rank = (int)cluster.block_rank();
         R.slots = slots;
         R.size = size;
-        R.base = team * (G.threads >> 5);
+        R.base = team * warps;
         R.team = team;
-        R.warp = t >> 5;
-        R.warps = G.threads >> 5;
+        R.warp = warp - team * warps;
+        R.warps = warps;
         R.lane = t & 31;
         R.parity = 0;
         const int c0 = R.rank * G.share;
@@ -440,6 +455,9 @@ struct Ring {
     }
 };
 
+// (rsqrtf: 2 units in the last place, where sums of a row's terms are off by more;
+// a square root and a quotient are 30 instructions that every thread repeats.)
+//
 // Mean and 1 / deviation of a row (mean 0 without `layer`); its values lose
 // their mean.
 template <int I, bool VECTOR>
@@ -465,7 +483,7 @@ __device__ __forceinline__ float2 statistics(Reducer& R, const Cols<VECTOR>& col
         for (int j = 0; j < 4; ++j) t = fma(v[i][j], v[i][j], t);
     float q[1] = {t.x + t.y};
     R.sum<0>(q);
-    return make_float2(mean, 1.0f / sqrtf(fmaf(q[0], inv, eps)));
+    return make_float2(mean, rsqrtf(fmaf(q[0], inv, eps)));
 }
 
 // RMS norm without biases, rows on 16-byte boundaries: rows go straight to
