@@ -527,16 +527,19 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
     HT* no = static_cast<HT*>(d.n) + r0 * d.dim;
     if (kKeep && r0 < r1) fetch();
     int64_t turn = r0;   // the row at which another row of the gate begins
+    const void* gate = d.gate;
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, no += d.dim) {
-        const void* gate = d.gate;
-        if (gate != nullptr && d.gate_rows > 1 && (!kKeep || r == turn))
-            gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
-        if (kKeep && r == turn) {
-            if (h != nullptr)
+        if (r == turn) {
+            turn = r1;
+            if (d.gate_rows > 1) {
+                const int64_t k = r / per;
+                gate = static_cast<const char*>(d.gate) + k * d.dim * (pb ? 2 : 4);
+                turn = (k + 1) * per;
+            }
+            if (kKeep && h != nullptr)
 #pragma unroll
                 for (int i = 0; i < I; ++i)
                     post_parameters<false>(d, gate, pb, cols.chunk(i), kp[kKeep ? i : 0], none);
-            turn = d.gate_rows > 1 ? (r / per + 1) * per : r1;
         }
         F8 v[I];
         Raw<XT, true> rx[I];
@@ -652,17 +655,20 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
     XT* xo = static_cast<XT*>(d.x_new) + r0 * d.dim;
     HT* no = static_cast<HT*>(d.n) + r0 * d.dim;
     int64_t turn = r0;   // the row at which another row of the gate begins
+    const void* gate = d.gate;
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, no += d.dim) {
-        const void* gate = d.gate;
-        if (gate != nullptr && d.gate_rows > 1 && (!kKeep || r == turn))
-            gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
-        if (kKeep && r == turn) {
-            if (has_h)
+        if (r == turn) {
+            turn = r1;
+            if (d.gate_rows > 1) {
+                const int64_t k = r / per;
+                gate = static_cast<const char*>(d.gate) + k * d.dim * (pb ? 2 : 4);
+                turn = (k + 1) * per;
+            }
+            if (kKeep && has_h)
 #pragma unroll
                 for (int i = 0; i < I; ++i)
                     post_parameters<FULL>(d, gate, pb, cols.chunk(i), kp[kKeep ? i : 0],
                                           kb[kKeep && FULL ? i : 0]);
-            turn = d.gate_rows > 1 ? (r / per + 1) * per : r1;
         }
         const char* s0 = ring.row(P.t);
         const HT* hr = reinterpret_cast<const HT*>(s0 + shifts[0]);
@@ -906,11 +912,15 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
     XT* xo = static_cast<XT*>(g.grad_x) + r0 * d.dim;
     HT* ho = static_cast<HT*>(g.grad_h) + r0 * d.dim;
     // The rows of every CTA of a cluster are the same, so all take part in its sums.
+    int64_t turn = r0, k0 = 0;   // the row at which another row of the gate begins; this one's
+    const void* gate = d.gate;
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, ho += d.dim) {
         fetch();
-        const void* gate = d.gate;
-        if (GROUPED && d.gate_rows > 1)
-            gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
+        if (GROUPED && r == turn) {
+            k0 = r / per;
+            gate = static_cast<const char*>(d.gate) + k0 * d.dim * (pb ? 2 : 4);
+            turn = (k0 + 1) * per;
+        }
         // hh, xh, e and p of a chunk; outside of the row e and p are 0
         const auto values = [&](int i, const Cols<VECTOR>& c, F8& hh, F8& xh, F8& e, F8& p) {
             F8 b;
@@ -1011,8 +1021,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_rows(const __grid_constant
             if (FULL) add_to(GROUPED ? 5 : kPostBias, c, t);
         }
         if constexpr (GROUPED) {
-            if (r + 1 == r1 || (r + 1) % per == 0) {   // the group ends, or this team's part of it
-                const int64_t k0 = r / per, first = k0 * per, last = first + per - 1;
+            if (r + 1 == r1 || r + 1 == turn) {   // the group ends, or this team's part of it
+                const int64_t first = k0 * per, last = first + per - 1;
                 const bool whole = first >= r0 && last < r1;
                 float* edge = W.edges + ((P.index * 2 + (first >= r0)) * 2) * d.dim;
 #pragma unroll
@@ -1112,16 +1122,19 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     XT* xo = static_cast<XT*>(g.grad_x) + r0 * d.dim;
     HT* ho = static_cast<HT*>(g.grad_h) + r0 * d.dim;
     const float a = has_h ? d.residual_scale : 1.0f;
-    int64_t turn = r0;   // the row at which another row of the gate begins
+    int64_t turn = r0, k0 = 0;   // the row at which another row of the gate begins; this one's
+    const void* gate = d.gate;
     // The rows of every CTA of a cluster are the same, so all take part in its sums.
     for (int64_t r = r0; r < r1; ++r, xo += d.dim, ho += d.dim) {
-        const void* gate = d.gate;
-        if (GROUPED) gate = static_cast<const char*>(gate) + r / per * d.dim * (pb ? 2 : 4);
         if (r == turn) {
+            if (GROUPED) {
+                k0 = r / per;
+                gate = static_cast<const char*>(d.gate) + k0 * d.dim * (pb ? 2 : 4);
+            }
             fill(kp, 0.0f);
             fill(kb, 0.0f);
             if (has_h) post_parameters<FULL>(d, gate, pb, cols, kp, kb);
-            turn = GROUPED ? (r / per + 1) * per : r1;
+            turn = GROUPED ? (k0 + 1) * per : r1;
         }
         const char* s0 = ring.row(P.t);
         const float4 st = ring.lost ? make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F)
@@ -1212,7 +1225,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
         }
         if constexpr (GROUPED) {
             if (r + 1 == r1 || r + 1 == turn) {   // the group ends, or this team's part of it
-                const int64_t k0 = r / per, first = k0 * per, last = first + per - 1;
+                const int64_t first = k0 * per, last = first + per - 1;
                 float* edge = nullptr;
                 if (first < r0 || last >= r1) edge = W.edges + ((P.index * 2 + (first >= r0)) * 2) * d.dim;
                 end_group<VECTOR, FULL>(g, gate, pb, cols, k0, edge, group, acc);
