@@ -289,21 +289,22 @@ int64_t stage_of(int64_t row_bytes, int arrays, bool vec, const Teams& G, int ch
     return vec ? row_bytes * G.share : row_bytes * G.threads * kCols * chunks + 48 * arrays;
 }
 // Teams of a CTA: as many as rows for all SMs need, 512 threads at most, and so
-// many stages for each that two rows are on their way, in 200 KB.
-bool plan_ring(int64_t rows, int64_t stage, bool one, Teams* G, int* stages, size_t* smem) {
+// many stages for each that two rows are on their way, in 200 KB with `kept` bytes
+// of each team beside its stages.
+bool plan_ring(int64_t rows, int64_t stage, int64_t kept, bool one, Teams* G, int* stages, size_t* smem) {
     const int64_t room = 200 * 1024;
     int64_t teams = one ? 1 : kTeam / G->threads;
     const int64_t need = ceil_div(rows, 148);
     if (teams > need) teams = need < 1 ? 1 : need;
-    while (teams > 1 && 3 * stage * teams > room) --teams;
-    int64_t n = room / (stage * teams);
+    while (teams > 1 && (3 * stage + kept) * teams > room) --teams;
+    int64_t n = (room / teams - kept) / stage;
     if (n < 2) return false;
     const int64_t run = ceil_div(rows, 148 * teams);   // more would not be used
     if (n > run + 1) n = run + 1 < 2 ? 2 : run + 1;
     if (n > kMaxStages) n = kMaxStages;
     G->teams = (int)teams;
     *stages = (int)n;
-    *smem = (size_t)(n * stage * teams);
+    *smem = (size_t)((n * stage + kept) * teams);
     return true;
 }
 
@@ -332,7 +333,7 @@ bool plan_forward(int64_t rows, int64_t dim, int64_t row_bytes, bool vec, bool f
         if (!ring) {
             G.teams = p->cluster > 1 || G.threads > 64 ? 1 : 128 / G.threads;
             if (G.threads * G.teams < kTeam) ctas = kTeam / (G.threads * G.teams);
-        } else if (!plan_ring(rows, stage_of(row_bytes, 2, vec, G, p->chunks), p->cluster > 1, &G,
+        } else if (!plan_ring(rows, stage_of(row_bytes, 2, vec, G, p->chunks), 0, p->cluster > 1, &G,
                               &p->stages, &p->smem)) {
             continue;   // a stage too large: more CTAs a row
         }
@@ -391,8 +392,10 @@ bool plan_stream(int64_t rows, int64_t dim, int64_t gate_rows, int64_t row_bytes
     Teams& G = p->G;
     G.threads = threads_for(G.share, 1);
     const int64_t stage = stage_of(row_bytes, 4, vec, G, 1) + 16;
-    if (!plan_ring(rows, stage, p->cluster > 1, &G, &p->stages, &p->smem)) return false;
-    const size_t sums = G.teams > 1 ? (full ? 4 : 2) * G.share * sizeof(float) : 0;
+    // a gate of groups: every thread's sums over its groups
+    const int64_t kept = gate_rows > 1 ? (full ? 64 : 32) * G.threads : 0;
+    if (!plan_ring(rows, stage, kept, p->cluster > 1, &G, &p->stages, &p->smem)) return false;
+    const size_t sums = kept * G.teams + (G.teams > 1 ? (full ? 4 : 2) * G.share * sizeof(float) : 0);
     if (p->smem < sums) p->smem = sums;
     plan_rows(rows, dim, gate_rows, p);
     return true;

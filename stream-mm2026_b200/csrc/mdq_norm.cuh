@@ -783,11 +783,13 @@ struct GradRaw {
 };
 
 // A group's sums of t hh and t leave the registers: the gate's gradient, or the
-// team's part of it, and their share of the parameters' gradients.
-template <bool VECTOR, bool FULL, int G, int A>
+// team's part of it, and their share of the parameters' gradients, which the thread
+// has in shared memory (`keep`, `step` floats apart): as they change with groups
+// only, registers for them would be taken from the rows.
+template <bool VECTOR, bool FULL, int G>
 __device__ __forceinline__ void end_group(const mdq_residual_norm_grad_desc& g, const void* gate, bool pb,
                                           const Cols<VECTOR>& c, int64_t k0, float* edge, F8 (&group)[G],
-                                          F8 (&acc)[A]) {
+                                          float* keep, int step) {
     const int64_t dim = g.f.dim;
     F8 w, w1, b1;
     parameters(gate, pb, c, 1.0f, w);
@@ -797,8 +799,8 @@ __device__ __forceinline__ void end_group(const mdq_residual_norm_grad_desc& g, 
     for (int k = 0; k < 8; ++k) {
         if (!c.has(k)) continue;
         const float sum = value(group[0], k), sum_b = value(group[G - 1], k);
-        set(acc[kPost], k, fmaf(value(w, k), sum, value(acc[kPost], k)));
-        if (FULL) set(acc[A - 1], k, fmaf(value(w, k), sum_b, value(acc[A - 1], k)));
+        keep[k * step] = fmaf(value(w, k), sum, keep[k * step]);
+        if (FULL) keep[(8 + k) * step] = fmaf(value(w, k), sum_b, keep[(8 + k) * step]);
         if (edge != nullptr) {
             edge[c.at(k)] = sum;
             edge[dim + c.at(k)] = sum_b;
@@ -1093,7 +1095,12 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
     constexpr int sizes[kFeeds] = {sizeof(HT), sizeof(XT), sizeof(HT), sizeof(XT), 4};
     const int parts[kFeeds + 1] = {0, at_x, at_gn, at_gx, at_st, stage_bytes};
     Ring<VECTOR> ring;
-    ring.stage0 = memory + (size_t)P.team * stages * stage_bytes;
+    // GROUPED: first each thread's sums over its groups
+    const int kept = GROUPED ? (FULL ? 16 : 8) * (int)sizeof(float) * blockDim.x : 0;
+    float* keep = reinterpret_cast<float*>(memory) + threadIdx.x;
+    if (GROUPED)
+        for (int k = 0; k < (FULL ? 16 : 8); ++k) keep[k * blockDim.x] = 0.0f;
+    ring.stage0 = memory + kept + (size_t)P.team * stages * stage_bytes;
     ring.full = full[P.team];
     ring.feeds = feeds[P.team];
     ring.stages = stages;
@@ -1228,7 +1235,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
                 const int64_t first = k0 * per, last = first + per - 1;
                 float* edge = nullptr;
                 if (first < r0 || last >= r1) edge = W.edges + ((P.index * 2 + (first >= r0)) * 2) * d.dim;
-                end_group<VECTOR, FULL>(g, gate, pb, cols, k0, edge, group, acc);
+                end_group<VECTOR, FULL>(g, gate, pb, cols, k0, edge, group, keep, blockDim.x);
             }
         }
         ring.next();
@@ -1238,8 +1245,15 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
                 shifts[k] = (shifts[k] + (unsigned)strides[k] * sizes[k]) & 15;
     }
     ring.close(P.t, r1 - r0);
+    if constexpr (GROUPED) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            set(acc[kPost], k, keep[k * blockDim.x]);
+            if (FULL) set(acc[kKinds - 1], k, keep[(8 + k) * blockDim.x]);
+        }
+    }
     __syncthreads();
-    end_sums<VECTOR, kKinds>(P, G, W, (int)d.dim, reinterpret_cast<float*>(memory), acc);
+    end_sums<VECTOR, kKinds>(P, G, W, (int)d.dim, reinterpret_cast<float*>(memory + kept), acc);
     if (P.R.ctas > 1) cg::this_cluster().sync();
 }
 
