@@ -1,5 +1,11 @@
 // mdq_distill.cu - distillation from a teacher's top logits: loss and gradient
 // (mdq_ops.h).
+//
+// Bound by memory when the logits are read once: a row stays in shared memory
+// between its sum and its gradient.  Few rows are split over clusters
+// (distill_cluster; 8 bf16 rows of 50257: 7.4 us), many go through persistent CTAs
+// whose warps run their copies ahead (distill_stream; 16384 such rows with the
+// gradient 598 us, 5.5 TB/s; 2048 fp32 rows of 32000, loss alone, 45 us, 5.8 TB/s).
 #include "mdq_ops.cuh"
 
 #include <cooperative_groups.h>
@@ -833,7 +839,7 @@ mdq_status run_rows(const mdq_topk_distill_desc& d, cudaStream_t stream) {
     // the other joins its warps; 16 and one CTA where a row fills more than half
     // of the shared memory; fewer warps for rows below 32 KB (4 KB a warp), and
     // as many CTAs as the registers take.
-    // 16x1024 rows of 50257 bf16: 601 us with 8 warps, 718 with 16.
+    // 16x1024 rows of 50257 bf16: 598 us (5.5 TB/s) with 8 warps, 718 with 16.
     StreamPlan P;
     P.warps = 1;
     while (P.warps < 8 && 16 * units >= (int64_t)P.warps * 2 * 4096) P.warps *= 2;

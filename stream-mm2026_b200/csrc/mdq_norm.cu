@@ -316,10 +316,10 @@ struct RowsPlan {
 };
 // Forward: two chunks a thread for many rows above 256 columns, one for narrow
 // or few (as few threads as 512 allow), four where that is not enough.
-// 32768 bf16 rows of 768 / 128 columns: 48 / 18 us with two chunks, 108 / 15 with one.
+// 32768 bf16 rows of 768 / 128 columns: 45 / 18 us with two chunks, 108 / 13 with one.
 // Four chunks have their parameters loaded for every row, value by value off 16
-// bytes: rather twice the CTAs then (4112 bf16 rows of 16301: 284 against 488 us),
-// but for fp32 rows without means and biases (6704 of 10001: 400 against 296).
+// bytes: rather twice the CTAs then (4112 bf16 rows of 16301: 244 against 553 us),
+// but for fp32 rows without means and biases (6704 of 10001: 355 against 287).
 bool plan_forward(int64_t rows, int64_t dim, int64_t row_bytes, bool vec, bool full, RowsPlan* p) {
     const bool ring = full || !vec;
     for (int most = vec || (row_bytes == 8 && !full) ? 4 : 2; most >= 1; most /= 2) {
@@ -382,8 +382,8 @@ bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, bool full, GradPlan
     return true;
 }
 // With rows in a ring.  Above 8192 columns the steps between more than two CTAs
-// take longer than the other kernel's rows (437 against 385 us for 4096 bf16 rows of
-// 16384), but not than its loads of rows off 16 bytes (571 against 2549 us for 4112
+// take longer than the other kernel's rows (440 against 312 us for 4096 bf16 rows of
+// 16384), but not than its loads of rows off 16 bytes (513 against 2549 us for 4112
 // rows of 16301).
 bool plan_stream(int64_t rows, int64_t dim, int64_t gate_rows, int64_t row_bytes, bool vec, bool full,
                  GradPlan* p) {
