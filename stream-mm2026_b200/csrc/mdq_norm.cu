@@ -316,7 +316,8 @@ struct RowsPlan {
 };
 // Forward: two chunks a thread for many rows above 256 columns, one for narrow
 // or few (as few threads as 512 allow), four where that is not enough.
-// 32768 bf16 rows of 768 / 128 columns: 45 / 18 us with two chunks, 108 / 13 with one.
+// 32768 bf16 rows of 2048 / 768 / 128 columns: 96 / 46 / 16 us with two chunks, 126 /
+// 81 / 13 with one, 112 / 50 / 32 with four.
 // Four chunks have their parameters loaded for every row, value by value off 16
 // bytes: rather twice the CTAs then (4112 bf16 rows of 16301: 244 against 553 us),
 // but for fp32 rows without means and biases (6704 of 10001: 355 against 287).
