@@ -514,7 +514,8 @@ def _entangled(a: torch.Tensor, b: torch.Tensor) -> bool:
     if rows == 0:
         return False
     off = b.data_ptr() - a.data_ptr()
-    sa, sb = ((_row_stride(t, "rows") if rows > 1 else 0) * size for t in (a, b))
+    sa, sb = ((_row_stride(t, what) if rows > 1 else 0) * size
+              for t, what in ((a, "logits"), (b, "out")))
     if off >= (rows - 1) * sa + vocab * size or -off >= (rows - 1) * sb + vocab * size:
         return False
     if sa != sb:
