@@ -114,7 +114,8 @@ mdq_status mdq_residual_norm(const mdq_residual_norm_desc* d, cudaStream_t strea
  * unrounded).  grad_new / grad_n may be NULL for zero.  grad_x and grad_h are
  * written contiguously in x_dtype and h_dtype, the parameters' gradients in
  * param_dtype; each is NULL where the forward argument was.  `f.x_new`, `f.n`
- * are unused.
+ * are unused.  Without rows the parameters' gradients are zeros and the
+ * workspace is not used.
  */
 typedef struct mdq_residual_norm_grad_desc {
     mdq_residual_norm_desc f;

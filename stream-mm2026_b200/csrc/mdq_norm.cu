@@ -2,6 +2,8 @@
 // and the kernels for rows that no cluster holds (the others: mdq_norm.cuh).
 #include "mdq_norm.cuh"
 
+#include <utility>
+
 namespace {
 
 using namespace mdq_norm;
@@ -494,6 +496,16 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: null pointer");
     if (!aligned16(g->workspace) || !aligned16(g->f.stats))
         return mdq_fail(MDQ_ERR_INVALID_ARG, "residual norm grad: workspace or stats misaligned");
+    if (g->f.rows == 0) {   // sums over no rows, whatever the parameters hold
+        const size_t row = (size_t)(g->f.dim * type_size(g->f.param_dtype));
+        const std::pair<void*, int64_t> sums[] = {
+            {g->grad_post_weight, 1}, {g->grad_post_bias, 1}, {g->grad_pre_weight, 1},
+            {g->grad_pre_bias, 1},    {g->grad_gate, g->f.gate_rows}};
+        cudaError_t e = cudaSuccess;
+        for (const auto& s : sums)
+            if (s.first != nullptr && e == cudaSuccess) e = cudaMemsetAsync(s.first, 0, s.second * row, stream);
+        return status_of(e, "residual norm grad");
+    }
     const bool grouped = g->f.gate_rows > 1;
     const bool full = g->f.kind == MDQ_NORM_LAYER || g->f.post_bias != nullptr || g->f.pre_bias != nullptr;
     const bool vec = vector_rows(g->f) && aligned16(g->grad_x) && aligned16(g->grad_h) &&
@@ -509,8 +521,7 @@ mdq_status mdq_residual_norm_grad(const mdq_residual_norm_grad_desc* g, cudaStre
                         (long long)g->workspace_bytes, (long long)need);
     if (!planned) {
         float* means = static_cast<float*>(g->workspace);
-        if (g->f.rows > 0)
-            norm_grad_wide<<<(unsigned)g->f.rows, kThreads, 0, stream>>>(*g, means);
+        norm_grad_wide<<<(unsigned)g->f.rows, kThreads, 0, stream>>>(*g, means);
         norm_grad_wide_columns<<<(unsigned)ceil_div(g->f.dim, kThreads), kThreads, 0, stream>>>(*g, means);
         return launch_status("residual norm grad");
     }
