@@ -24,6 +24,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -198,7 +199,8 @@ def scaled_embedding_grad(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int,
     if padding_idx is not None and not 0 <= padding_idx < vocab:
         raise RuntimeError("padding_idx must lie in [0, vocab)")
     stride = _row_stride(grad_out, "grad_out")
-    if out is None:
+    given = out is not None
+    if not given:
         if accumulate:
             raise RuntimeError("accumulate needs out")
         out = _empty((vocab, dim), (dim, 1), dtype, grad_out.device)
@@ -214,6 +216,8 @@ def scaled_embedding_grad(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int,
         grad_out.data_ptr(), ids.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes, tokens, vocab, dim,
         stride, -1 if padding_idx is None else padding_idx, scale, go_code, out_code, ids_code,
         1 if accumulate else 0, 0))
+    if given:
+        increment_version(out)   # backward passes that need its former values refuse
     return out
 
 
@@ -544,7 +548,8 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     ``out`` receives the gradient (logits' shape and dtype, evenly strided rows);
     it may be ``logits``, which are then overwritten, but share nothing else with them.  Without ``grad`` only the
     loss is computed."""
-    if out is not None:
+    given = out is not None
+    if given:
         if not grad:
             raise RuntimeError("out needs grad")
         _on(out, _device(logits, "logits"), "out")
@@ -559,6 +564,8 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
         out = _like(logits)
     total, losses = _distill(logits, teacher_logits, teacher_index, temperature, weight,
                              scale, out)
+    if given:
+        increment_version(out)   # backward passes that need its former values refuse
     return TopkDistill(total, losses, out)
 
 

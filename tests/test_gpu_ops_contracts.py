@@ -1,12 +1,13 @@
 """What callers of the training-step operators rely on beside the values: calls
-without rows through the C ABI.
+without rows through the C ABI, and results written into a caller's tensor,
+which autograd has to learn of.
 """
 import ctypes
 
 import pytest
 import torch
 
-from mdq_b200 import _lib
+from mdq_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,48 @@ def test_residual_norm_grad_without_rows(cuda_device, groups, kind, dim):
     assert lib.mdq_residual_norm_grad(ctypes.byref(g), stream) == 0
     for k, t in grads.items():
         assert bool((t == 0).all()), k
+
+
+def _distill_into(out, dev):
+    rows = out.shape[0]
+    return ops.topk_distill(out, torch.zeros(rows, 2, device=dev),
+                            torch.zeros(rows, 2, dtype=torch.int64, device=dev), out=out).grad
+
+
+def _sums_into(accumulate):
+    def write(out, dev):
+        ids = torch.arange(out.shape[0], device=dev)
+        return ops.scaled_embedding_grad(ids, torch.ones_like(out), out.shape[0], out=out,
+                                         accumulate=accumulate)
+    return write
+
+
+@pytest.mark.parametrize("write", [_distill_into, _sums_into(False), _sums_into(True)],
+                         ids=["distill", "embedding", "embedding added"])
+def test_results_in_a_callers_tensor_raise_its_version(cuda_device, write):
+    """As an in-place operation of torch: a backward pass that needs the values
+    that were overwritten refuses."""
+    leaf = torch.randn(6, 40, device=cuda_device, requires_grad=True)
+    saved = torch.exp(leaf)            # its backward pass reads the result
+    out = saved.detach()
+    version = out._version
+    assert write(out, cuda_device) is out
+    assert out._version == version + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.sum().backward()
+    # the logits that the loss's own backward pass reads
+    logits = torch.randn(6, 40, device=cuda_device, requires_grad=True)
+    loss = ops.topk_distill_loss(logits, torch.zeros(6, 1, device=cuda_device),
+                                 torch.zeros(6, 1, dtype=torch.int64, device=cuda_device))
+    write(logits.detach(), cuda_device)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    # a refused call has written nothing; inference tensors have no version
+    version = out._version
+    with pytest.raises(RuntimeError, match="temperature"):
+        ops.topk_distill(out, out[:, :2].contiguous(),
+                         torch.zeros(6, 2, dtype=torch.int64, device=cuda_device),
+                         temperature=0.0, out=out)
+    assert out._version == version
+    with torch.inference_mode():
+        assert bool(torch.isfinite(write(torch.randn(6, 40, device=cuda_device), cuda_device)).all())
