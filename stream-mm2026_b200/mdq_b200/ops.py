@@ -10,10 +10,11 @@ language model's step, as CUDA kernels behind the C ABI of ``include/mdq_ops.h``
 
 ``scaled_embedding``, ``residual_norm`` and ``topk_distill_loss`` take part in
 autograd; the others are the passes themselves, for programs that run their own
-backward.  Every call works on the current stream of its tensors' device,
-allocates its results and scratch through torch's caching allocator and does not
-wait for the device.  Tensors are float32 or bfloat16; the last dimension is
-contiguous and rows may be strided.  CPU tensors are refused.
+backward.  There is no forward-mode derivative: dual tensors are refused.  Every
+call works on the current stream of its tensors' device, allocates its results and
+scratch through torch's caching allocator and does not wait for the device.
+Tensors are float32 or bfloat16; the last dimension is contiguous and rows may be
+strided.  CPU tensors are refused.
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -63,6 +65,15 @@ def _device(t: torch.Tensor, what: str) -> int:
 def _on(t: torch.Tensor, index: int, what: str) -> None:
     if t.get_device() != index:
         raise RuntimeError(f"{what} must be on cuda:{index}")
+
+
+def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors with a forward-mode tangent, which the kernels do not see."""
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the operators have no forward-mode derivative")
 
 
 def _row_stride(t: torch.Tensor, what: str) -> int:
@@ -163,6 +174,7 @@ def _check_ids(ids: torch.Tensor, dev: int) -> int:
 
 def _embedding_forward(ids, table, scale, out_dtype):
     dev = _device(table, "table")
+    _no_tangents(table)
     if table.dim() != 2 or table.numel() == 0:
         raise RuntimeError("table must be [vocab, dim], neither of them 0")
     ids_code, table_code = _check_ids(ids, dev), _float_code(table, "table")
@@ -190,6 +202,7 @@ def scaled_embedding_grad(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int,
     (fp32) the sums are added to it, and only the rows that occur are touched.
     """
     dev = _device(grad_out, "grad_out")
+    _no_tangents(grad_out, out)
     ids_code, go_code = _check_ids(ids, dev), _float_code(grad_out, "grad_out")
     if grad_out.dim() < 1 or grad_out.shape[:-1] != ids.shape:
         raise RuntimeError("grad_out must be [*ids.shape, dim]")
@@ -347,6 +360,7 @@ def residual_norm_forward(x, h, post_weight, pre_weight, *, post_bias=None, pre_
     4] fp32) is what ``residual_norm_backward`` needs, None without
     ``want_stats``."""
     _device(x, "x")
+    _no_tangents(x, h, post_weight, pre_weight, post_bias, pre_bias, gate)
     x_new = x if h is None else _like(x)
     n = None
     if pre_weight is not None:
@@ -371,6 +385,7 @@ def residual_norm_backward(grad_new, grad_n, x, h, stats, post_weight, pre_weigh
     if stats is None or stats.dtype != torch.float32 or not stats.is_contiguous() or \
             stats.numel() != 4 * _row_count(x):
         raise RuntimeError("stats must be the forward pass's")
+    _no_tangents(grad_new, grad_n, x, h, stats, post_weight, pre_weight, post_bias, pre_bias, gate)
     dev, fields = _norm_fields(x, h, post_weight, pre_weight, post_bias, pre_bias, gate,
                                residual_scale, 0.0, kind, None, None, stats)
     _on(stats, dev, "stats")
@@ -471,6 +486,7 @@ class TopkDistill(NamedTuple):
 def _distill(logits, teacher, index, temperature, weight, scale, grad, upstream=None,
              want_loss=True):
     dev = _device(logits, "logits")
+    _no_tangents(logits, teacher, weight, grad, upstream)
     code, t_code = _float_code(logits, "logits"), _float_code(teacher, "teacher_logits")
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise RuntimeError("logits must be [..., vocab]")

@@ -1,11 +1,12 @@
 """What callers of the training-step operators rely on beside the values: calls
-without rows through the C ABI, and results written into a caller's tensor,
-which autograd has to learn of.
+without rows through the C ABI, results written into a caller's tensor,
+which autograd has to learn of, and forward-mode tangents.
 """
 import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from mdq_b200 import _lib, ops
 
@@ -86,3 +87,52 @@ def test_results_in_a_callers_tensor_raise_its_version(cuda_device, write):
     assert out._version == version
     with torch.inference_mode():
         assert bool(torch.isfinite(write(torch.randn(6, 40, device=cuda_device), cuda_device)).all())
+
+
+def _calls_with(dev):
+    """Every front end, as a function of one of its floating-point arguments."""
+    x, h = torch.randn(6, 40, device=dev), torch.randn(6, 40, device=dev)
+    w, ids = torch.ones(40, device=dev), torch.arange(6, device=dev)
+    t, at = torch.zeros(6, 2, device=dev), torch.zeros(6, 2, dtype=torch.int64, device=dev)
+    weight = torch.ones(6, device=dev)
+    stats = ops.residual_norm_forward(x, h, w, w)[2]
+    return {
+        "embedding": (x, lambda v: ops.scaled_embedding(ids, v)),
+        "embedding grad": (x, lambda v: ops.scaled_embedding_grad(ids, v, 6)),
+        "embedding grad out": (x, lambda v: ops.scaled_embedding_grad(ids, x, 6, out=v)),
+        "norm x": (x, lambda v: ops.residual_norm(v, h, w, w)),
+        "norm h": (x, lambda v: ops.residual_norm(x, v, w, w)),
+        "norm first": (x, lambda v: ops.residual_norm(v, None, None, w)),
+        "norm weight": (w, lambda v: ops.residual_norm(x, h, v, w)),
+        "norm bias": (w, lambda v: ops.residual_norm(x, h, w, w, pre_bias=v)),
+        "norm gate": (w, lambda v: ops.residual_norm_forward(x, h, w, w, gate=v)),
+        "norm backward": (x, lambda v: ops.residual_norm_backward(v, x, x, h, stats, w, w)),
+        "norm backward stats": (stats, lambda v: ops.residual_norm_backward(x, x, x, h, v, w, w)),
+        "distill": (x, lambda v: ops.topk_distill(v, t, at)),
+        "distill teacher": (t, lambda v: ops.topk_distill_loss(x, v, at)),
+        "distill weight": (weight, lambda v: ops.topk_distill(x, t, at, weight=v)),
+        "distill out": (x, lambda v: ops.topk_distill(x, t, at, out=v)),
+        "distill loss": (x, lambda v: ops.topk_distill_loss(v, t, at)),
+    }
+
+
+def test_forward_mode_tangents_are_refused(cuda_device):
+    """No operator has a forward-mode derivative: a dual tensor is refused, with or
+    without reverse mode, and not taken for its primal."""
+    for name, (value, call) in _calls_with(cuda_device).items():
+        call(value.clone())
+        with forward_ad.dual_level():
+            call(value.clone())                   # no tangent: as ever
+            for grad in (False, True):
+                dual = forward_ad.make_dual(value.clone().requires_grad_(grad),
+                                            torch.ones_like(value))
+                with pytest.raises(RuntimeError, match="forward"):
+                    call(dual)
+                    pytest.fail(name)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+                    call(dual)
+                    pytest.fail(name)
+    # and under torch.func, whose tensors have no memory of their own
+    x, w = torch.randn(6, 40, device=cuda_device), torch.ones(40, device=cuda_device)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: ops.residual_norm(v, None, None, w)[1], (x,), (x,))
