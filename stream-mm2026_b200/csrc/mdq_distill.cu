@@ -406,7 +406,10 @@ __global__ void __launch_bounds__(kThreads, 2) distill_cluster(const __grid_cons
             arrived &= bar_wait(&S.bar[k], 0);
             if (live) add_units<T>(a, units, k * per + tid, min(n, (k + 1) * per), threads, c);
         }
-    if (!arrived) a.s = CUDART_NAN_F;   // the row's results become NaN
+    if (!arrived) {   // the row's results become NaN; copies still on their way end in this CTA's time
+        a.s = CUDART_NAN_F;
+        for (int k = 0; k < kParts; ++k) (void)bar_wait(&S.bar[k], 0);
+    }
     // All threads, all CTAs.
     a = merge_warp(a);
     if (lane == 0) S.warp[warp] = a;
@@ -467,8 +470,10 @@ struct StreamPlan {
 };
 constexpr int kMaxStages = 8, kMaxDepth = 4;
 
-// Waits that ran out.
-__device__ unsigned int g_distill_timeouts;
+// A wait of a whole warp.
+[[nodiscard]] __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity));
+}
 
 // A place in a ring: its stage, and the phase its barriers are in.
 struct Place {
@@ -578,13 +583,17 @@ __device__ __forceinline__ void stream_entries(const mdq_topk_distill_desc& d, c
                                                int lane) {
     const float c = 1.0f / d.temperature * kLog2e;
     Place slots;
-    // The loss of the row whose entries are in the slot, once the others are done.
-    const auto finish = [&](int slot, int64_t r, unsigned phase) {
-        if (!bar_wait(&S.heard[slot], phase)) {
-            if (lane == 0) atomicAdd(&g_distill_timeouts, 1u);
+    // The loss of row i, whose entries are in the slot, once the others are done.  If
+    // they do not come, this warp ends (theirs do after a wait for their next entries),
+    // and the losses from here on are NaN.
+    const auto finish = [&](int slot, int64_t i, unsigned phase) {
+        const bool done = warp_wait(&S.heard[slot], phase);
+        if (d.row_loss == nullptr) return done;
+        if (!done) {
+            for (i += lane; i < R.live; i += 32) d.row_loss[R.at(i)] = CUDART_NAN_F;
             return false;
         }
-        if (d.row_loss == nullptr) return true;
+        const int64_t r = R.at(i);
         const Teacher K(info + (size_t)slot * kTeacherBytes * d.top, d.top);
         float l = 0.0f;
         if (S.live[slot])
@@ -594,10 +603,12 @@ __device__ __forceinline__ void stream_entries(const mdq_topk_distill_desc& d, c
         __syncwarp();
         return true;
     };
+    if (d.row_loss != nullptr)
+        for (int64_t i = lane; i < R.dead; i += 32) d.row_loss[R.at(R.live + i)] = 0.0f;
     for (int64_t i = 0; i < R.live; ++i) {
         const int64_t r = R.at(i);
         const int slot = slots.stage;
-        if (i >= P.depth && !finish(slot, R.at(i - P.depth), slots.phase ^ 1)) return;
+        if (i >= P.depth && !finish(slot, i - P.depth, slots.phase ^ 1)) return;
         const Teacher K(info + (size_t)slot * kTeacherBytes * d.top, d.top);
         const T* z = static_cast<const T*>(d.logits) + r * d.logits_stride;
         const bool live = row_weight(d, r) != 0.0f &&
@@ -608,10 +619,9 @@ __device__ __forceinline__ void stream_entries(const mdq_topk_distill_desc& d, c
         slots.next(P.depth);
     }
     if (d.row_loss == nullptr) return;
-    for (int64_t i = lane; i < R.dead; i += 32) d.row_loss[R.at(R.live + i)] = 0.0f;
     if (R.live < P.depth) slots = {0, 1};
     for (int64_t i = max((int64_t)0, R.live - P.depth); i < R.live; ++i, slots.next(P.depth))
-        if (!finish(slots.stage, R.at(i), slots.phase ^ 1)) return;
+        if (!finish(slots.stage, i, slots.phase ^ 1)) return;
 }
 
 template <typename T>
@@ -658,7 +668,11 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
     int64_t inext = 0;
     int ik = 0, loads = 0, in = 0, iunits = 0;
     Place to;
+    // A wait of this warp ran out: it waits for nothing and copies nothing from then
+    // on, what it has to write becomes NaN, and through its sums all of the rows do.
+    bool lost = false;
     const auto copy_next = [&] {
+        if (lost) return;
         while (ik == loads) {
             if (inext == R.live) return;
             const Share<T> s(d, logits + R.at(inext) * d.logits_stride, first, P.each);
@@ -701,9 +715,11 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
         const int n = pieces_of(s.mine), keep = want ? min(n, P.stages) : 0;
         const Place begin = at;
         Stat a = {-CUDART_INF_F, 0.0f};
-        bool arrived = true;
-        for (int k = 0; k < n; ++k, at.next(P.stages)) {
-            arrived &= bar_wait(&S.full[warp][at.stage], at.phase);
+        for (int k = 0; k < n && !lost; ++k, at.next(P.stages)) {
+            if (!warp_wait(&S.full[warp][at.stage], at.phase)) {
+                lost = true;
+                break;
+            }
             add_units<T>(a, reinterpret_cast<const uint4*>(ring + at.stage * piece_bytes), lane,
                          min(P.piece_units, s.mine - k * P.piece_units), 32, c);
             if (k < n - keep) {
@@ -716,11 +732,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
             a = merge(a, {h, ex2(fmaf(edge_value, c, -finite_max(h)))});
         }
         const int slot = slots.stage;
-        arrived &= bar_wait(&S.told[slot], slots.phase);
-        if (!arrived) {   // the row's results become NaN
-            a.s = CUDART_NAN_F;
-            if (lane == 0) atomicAdd(&g_distill_timeouts, 1u);
-        }
+        if (!lost && !warp_wait(&S.told[slot], slots.phase)) lost = true;
+        if (lost) a.s = CUDART_NAN_F;
         a = merge_warp(a);
         if (lane == 0) S.warp[parity][warp] = a;
         asm volatile("bar.sync 1, %0;" ::"r"(32 * W) : "memory");
@@ -730,7 +743,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
 
         if (want) {
             // ---- gradient: the pieces in the ring, then those brought again
-            const bool live = S.live[slot] != 0;
+            const bool live = !lost && S.live[slot] != 0;
             const float up = d.upstream == nullptr ? 1.0f : __ldg(d.upstream + r * d.upstream_stride);
             const float f = up * d.scale * w * d.temperature, pe = __fdividef(f, a.s);
             const float shift = finite_max(a.h);
@@ -739,12 +752,12 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
             const int end = s.from + s.mine * N;
             const auto entry = [&](int k, int& i, float& v) {
                 i = -1;
-                if (k >= d.top) return;
+                if (!live || k >= d.top) return;
                 const int at_index = K.idx[k];
                 const float sum = K.sum[k];
                 const bool own = (at_index >= s.from && at_index < end) ||
                                  (warp == 0 && (at_index < s.head || at_index >= (int)d.vocab - s.tail));
-                if (sum < 0.0f || !own || !live) return;
+                if (sum < 0.0f || !own) return;
                 i = at_index;
                 v = pe * ex2(fmaf(K.z[k], c, -shift)) - f * sum;
             };
@@ -759,16 +772,18 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
             for (int k = 0; k < n; ++k) {
                 const int piece = k < keep ? n - keep + k : k - keep;
                 const int stage = k < keep ? kept.stage : at.stage;
-                if (k < keep) {
+                if (k < keep)
                     kept.next(P.stages);
-                } else {
-                    bar_wait(&S.full[warp][stage], at.phase);
+                else if (!lost && warp_wait(&S.full[warp][stage], at.phase))
                     at.next(P.stages);
-                }
+                else
+                    lost = true;
                 const int u0 = piece * P.piece_units, count = min(P.piece_units, s.mine - u0);
                 const char* part = ring + stage * piece_bytes;
                 T* dst = mine + (int64_t)u0 * N;
-                if (!live) {
+                if (lost) {
+                    for (int j = lane; j < count * N; j += 32) dst[j] = from_f<T>(CUDART_NAN_F);
+                } else if (!live) {
                     write_zeros(dst, (int64_t)count * N, lane, 32);
                 } else if (same) {
                     const uint4* units = reinterpret_cast<const uint4*>(part);
@@ -787,7 +802,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
                 __syncwarp();
                 copy_next();
             }
-            if (edge) out[edge_at] = from_f<T>(live ? pe * ex2(fmaf(edge_value, c, -shift)) : 0.0f);
+            if (edge) out[edge_at] = from_f<T>(lost ? CUDART_NAN_F : live ? pe * ex2(fmaf(edge_value, c, -shift)) : 0.0f);
             __syncwarp();
             // The entries, over what was stored there.
             if (entry_at >= 0) out[entry_at] = from_f<T>(entry_value);
@@ -800,6 +815,9 @@ __global__ void __launch_bounds__(kThreads + 32, 1) distill_stream(const __grid_
         if (lane == 0) bar_arrive(&S.heard[slot]);
         slots.next(P.depth);
     }
+    if (lost)   // copies still on their way end in this CTA's time
+        for (; at.stage != to.stage || at.phase != to.phase; at.next(P.stages))
+            (void)bar_wait(&S.full[warp][at.stage], at.phase);
 }
 
 // The sum of the rows' losses, in a fixed order.
