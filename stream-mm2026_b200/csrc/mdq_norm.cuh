@@ -312,9 +312,6 @@ struct Place {
 
 constexpr int kMaxStages = 6;
 
-// Waits for copies that ran out.
-static __device__ unsigned int g_norm_timeouts;
-
 // A chunk's eight values in shared memory, the row's first at `row`.
 template <typename T, bool VECTOR>
 __device__ __forceinline__ void from_shared(const T* row, int at, F8& v) {
@@ -425,7 +422,7 @@ struct Ring {
     }
     // Behind that barrier, by the team's first warp: the next row into the next stage.
     __device__ __forceinline__ void copy_row(int t) {
-        if (left == 0) return;
+        if (left == 0 || lost) return;
         if (feeder) feed_row<VECTOR>(feeds[t], stage0 + to * stage_bytes, &full[to], policy);
         --left;
         if (++to == stages) to = 0;
@@ -436,26 +433,27 @@ struct Ring {
         if (t < 32)
             for (int k = 0; k < stages - 1; ++k) copy_row(t);
     }
-    // The present row's stage, once it is there; after a wait that ran out the
-    // results are made NaN (`lost`).
-    __device__ __forceinline__ const char* row(int t) {
-        if (!lost && !bar_wait(&full[stage], phase)) {
-            lost = true;
-            if (t == 0) atomicAdd(&g_norm_timeouts, 1u);
-        }
+    // The present row's stage, once it is there.  After a wait that ran out (`lost`)
+    // nothing is waited for or copied any more, the stage stays, and the thread's
+    // values of the rows are taken as NaN: through the sums all of the rows become it.
+    __device__ __forceinline__ const char* row() {
+        if (!lost && !bar_wait(&full[stage], phase)) lost = true;
         return stage0 + stage * stage_bytes;
     }
     __device__ __forceinline__ void next() {
-        if (++stage == stages) {
+        if (!lost && ++stage == stages) {
             stage = 0;
             phase ^= 1;
         }
     }
-    // Copies still on their way end before the CTA does.
-    __device__ __forceinline__ void close(int t, int64_t rows) {
-        if (lost && t == 0)
-            for (int64_t k = max((int64_t)0, rows - stages); k < rows; ++k)
-                bar_wait(&full[k % stages], (unsigned)(k / stages) & 1);
+    // Copies still on their way end before the CTA does: by the lanes that asked for
+    // them, from the row that was waited for up to their last.
+    __device__ __forceinline__ void close(int t) {
+        if (lost && t < 32 && feeder)
+            for (; stage != to; phase ^= stage == 0) {
+                (void)bar_wait(&full[stage], phase);
+                if (++stage == stages) stage = 0;
+            }
     }
 };
 
@@ -675,7 +673,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
                     post_parameters<FULL>(d, gate, pb, cols.chunk(i), kp[kKeep ? i : 0],
                                           kb[kKeep && FULL ? i : 0]);
         }
-        const char* s0 = ring.row(P.t);
+        const char* s0 = ring.row();
         const HT* hr = reinterpret_cast<const HT*>(s0 + shifts[0]);
         const XT* xr = reinterpret_cast<const XT*>(s0 + hb + shifts[1]);
         F8 v[I];
@@ -692,9 +690,9 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
                 from_shared<HT, VECTOR>(hr, place(i), v[i]);
                 if (ragged) within_row(v[i], cols.chunk(i));
             }
-            float2 s = statistics<I>(P.R, cols, v, layer, ragged, inv, d.eps);
+            if (ring.lost) v[0][0] = both(CUDART_NAN_F);
+            const float2 s = statistics<I>(P.R, cols, v, layer, ragged, inv, d.eps);
             refill();
-            if (ring.lost) s.y = CUDART_NAN_F;
             st.x = s.x;
             st.y = s.y;
 #pragma unroll
@@ -727,11 +725,11 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
                 from_shared<XT, VECTOR>(xr, place(i), v[i]);
                 if (ragged) within_row(v[i], cols.chunk(i));
             }
+            if (ring.lost) v[0][0] = both(CUDART_NAN_F);
         }
         if (d.n != nullptr) {
-            float2 s = statistics<I>(P.R, cols, v, layer, ragged, inv, d.eps);
+            const float2 s = statistics<I>(P.R, cols, v, layer, ragged, inv, d.eps);
             if (!has_h) refill();
-            if (ring.lost) s.y = CUDART_NAN_F;
             st.z = s.x;
             st.w = s.y;
 #pragma unroll
@@ -764,7 +762,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant
 #pragma unroll
             for (int k = 0; k < 2; ++k) shifts[k] = (shifts[k] + (unsigned)strides[k] * sizes[k]) & 15;
     }
-    ring.close(P.t, r1 - r0);
+    ring.close(P.t);
     if (P.R.ctas > 1) cg::this_cluster().sync();   // none ends while its memory may be written to
 }
 
@@ -1148,7 +1146,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
             if (has_h) post_parameters<FULL>(d, gate, pb, cols, kp, kb);
             turn = GROUPED ? (k0 + 1) * per : r1;
         }
-        const char* s0 = ring.row(P.t);
+        const char* s0 = ring.row();
         const float4 st = ring.lost ? make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F)
                                     : *reinterpret_cast<const float4*>(s0 + at_st);
         F8 hh, xh, dx, dn;
@@ -1249,7 +1247,7 @@ __global__ void __launch_bounds__(kTeam, 1) norm_grad_stream(const __grid_consta
             for (int k = 0; k < 4; ++k)
                 shifts[k] = (shifts[k] + (unsigned)strides[k] * sizes[k]) & 15;
     }
-    ring.close(P.t, r1 - r0);
+    ring.close(P.t);
     if constexpr (GROUPED) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
