@@ -84,8 +84,9 @@ def train(steps: int = 200, vocab: int = 512, dim: int = 128, layers: int = 2, h
     device = torch.device("cuda")
     model = SmallLM(vocab, dim, layers, heads).to(device)
     teacher = Teacher(vocab, top, device)
+    # (the optimizer's time constant grows with the logarithm of the layers, which is 0 for one)
     optimizer = MDQAdamWSimpleFusedIO(model.parameters(), lr=lr, weight_decay=0.0, block_size=256,
-                                      layer_count=layers, batch_size=batch)
+                                      layer_count=max(2, layers), batch_size=batch)
     losses = []
     for step in range(steps):
         ids = torch.randint(0, vocab, (batch, length), device=device)

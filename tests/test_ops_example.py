@@ -33,6 +33,12 @@ def test_example_learns(cuda_device):
 
 
 @pytest.mark.gpu
+def test_example_trains_one_layer(cuda_device):
+    losses = _example().train(steps=2, vocab=32, dim=32, layers=1, heads=2, batch=3, length=16, top=4, every=0)
+    assert len(losses) == 2 and all(math.isfinite(v) for v in losses)
+
+
+@pytest.mark.gpu
 def test_example_gradients(cuda_device):
     """The model's gradients on the operators against the same model on plain
     fp32 torch operations (bf16 products in both)."""
