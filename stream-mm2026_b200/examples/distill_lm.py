@@ -87,15 +87,15 @@ def train(steps: int = 200, vocab: int = 512, dim: int = 128, layers: int = 2, h
     # (the optimizer's time constant grows with the logarithm of the layers, which is 0 for one)
     optimizer = MDQAdamWSimpleFusedIO(model.parameters(), lr=lr, weight_decay=0.0, block_size=256,
                                       layer_count=max(2, layers), batch_size=batch)
-    losses = []
+    losses, padded = [], length // 8
     for step in range(steps):
         ids = torch.randint(0, vocab, (batch, length), device=device)
         weight = torch.ones(batch, length, device=device)
-        weight[:, -length // 8:] = 0          # as a batch's padding would be
+        weight[:, length - padded:] = 0       # as a batch's padding would be
         logits = model(ids)
         at = logits.detach()
         result = ops.topk_distill(at, *teacher(ids), temperature=temperature, weight=weight,
-                                  scale=1.0 / (batch * (length - length // 8)), out=at)
+                                  scale=1.0 / (batch * (length - padded)), out=at)
         logits.backward(result.grad)
         optimizer.step()
         optimizer.zero_grad()

@@ -39,6 +39,22 @@ def test_example_trains_one_layer(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("length", [1, 7, 9, 60, 64])
+def test_example_weights_add_up_to_one(cuda_device, length, monkeypatch):
+    """The loss is a mean: the weights of the positions that count, times the scale, sum to 1."""
+    m, seen = _example(), []
+
+    def look(*args, weight, scale, **kw):
+        seen.append(float(weight.sum()) * scale)
+        return distill(*args, weight=weight, scale=scale, **kw)
+
+    distill = m.ops.topk_distill
+    monkeypatch.setattr(m.ops, "topk_distill", look)
+    losses = m.train(steps=1, vocab=32, dim=32, layers=1, heads=2, batch=3, length=length, top=4, every=0)
+    assert math.isfinite(losses[0]) and seen == [pytest.approx(1.0, rel=1e-6)]
+
+
+@pytest.mark.gpu
 def test_example_gradients(cuda_device):
     """The model's gradients on the operators against the same model on plain
     fp32 torch operations (bf16 products in both)."""
