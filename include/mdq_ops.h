@@ -52,8 +52,9 @@ mdq_status mdq_embed(const mdq_embed_desc* d, cudaStream_t stream);
  * grad_out[n, :], in ascending order of n within fixed groups (the same bits on
  * every call).  Rows of ids that do not occur are written as zeros; with
  * `accumulate` (fp32 grad only) the sums are added to `grad` instead and other
- * rows are not touched.  Ids outside [0, vocab) and ids equal to padding_idx
- * (-1: none) contribute nothing.  tokens < 2^31.
+ * rows are not touched.  The addition to `grad` is the L2 cache's, which takes
+ * subnormal values as zero (below 1.2e-38 in magnitude).  Ids outside [0, vocab)
+ * and ids equal to padding_idx (-1: none) contribute nothing.  tokens < 2^31.
  */
 typedef struct mdq_embed_grad_desc {
     const void* grad_out;   /* [tokens, dim], grad_out_dtype, rows stride apart    */

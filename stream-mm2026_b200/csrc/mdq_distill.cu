@@ -3,9 +3,9 @@
 //
 // Bound by memory when the logits are read once: a row stays in shared memory
 // between its sum and its gradient.  Few rows are split over clusters
-// (distill_cluster; 8 bf16 rows of 50257: 7.4 us), many go through persistent CTAs
+// (distill_cluster; 8 bf16 rows of 50257: 7.3 us), many go through persistent CTAs
 // whose warps run their copies ahead (distill_stream; 16384 such rows with the
-// gradient 598 us, 5.5 TB/s; 2048 fp32 rows of 32000, loss alone, 45 us, 5.8 TB/s).
+// gradient 605 us, 5.4 TB/s; 2048 fp32 rows of 32000, loss alone, 45 us, 5.8 TB/s).
 #include "mdq_ops.cuh"
 
 #include <cooperative_groups.h>
@@ -33,7 +33,8 @@ __device__ __forceinline__ float finite_max(float h) { return h == -CUDART_INF_F
 
 // Softmax statistics: the largest exponent h = z c (rounded) and the sum of
 // exp2(z c - h).  Sums are rescaled by the difference of the rounded exponents
-// themselves, so that their rounding cancels.
+// themselves, so that their rounding cancels.  c = log2(e) / T is rounded to fp32: a
+// probability is off by about 1e-7 of itself times its exponent's distance from h.
 struct Stat {
     float h, s;
 };
@@ -857,7 +858,8 @@ mdq_status run_rows(const mdq_topk_distill_desc& d, cudaStream_t stream) {
     // the other joins its warps; 16 and one CTA where a row fills more than half
     // of the shared memory; fewer warps for rows below 32 KB (4 KB a warp), and
     // as many CTAs as the registers take.
-    // 16x1024 rows of 50257 bf16: 598 us (5.5 TB/s) with 8 warps, 718 with 16.
+    // 16x1024 rows of 50257 bf16: 605 us (5.4 TB/s) with 8 warps; when both were built
+    // 598, and 718 with 16.
     StreamPlan P;
     P.warps = 1;
     while (P.warps < 8 && 16 * units >= (int64_t)P.warps * 2 * 4096) P.warps *= 2;

@@ -18,11 +18,12 @@
 //   embed_grad_join   adds the partial sums of the runs that cross edges
 // A few tokens take one launch (embed_grad_few).
 //
-// Measured, bf16 rows and f32 tables: lookup of 8192 rows of 4096, 21.8 us (9.2 TB/s:
-// repeated ids come from L2), of 16384 rows of 768, 8.4; gradient of the latter into a
-// dense 50257 x 768 result 23.7 (sort, under 154 MB of zeros at 6.5 TB/s) + 12.1 + 5.7;
-// of the former added to a 128256 x 4096 gradient 8.5 (sort) + 40.6 + 8.7, for 201 MB
-// at least of rows read and added to.
+// Measured, bf16 rows and f32 tables, ids by word frequency: lookup of 8192 rows of
+// 4096 from 32000, 22.0 us (9.2 TB/s: repeated ids come from L2), of 16384 rows of 768,
+// 8.5; gradient of the latter into a dense 50257 x 768 result 23.6 (sort, under 154 MB
+// of zeros at 6.5 TB/s) + 12.1 + 5.8; of the former added to a 32000 x 4096 gradient 8.5
+// (sort) + 41.3 + 9.0, for 67 MB of rows and the 3264 rows of the gradient that occur,
+// 53 MB read and 53 written.
 #include "mdq_ops.cuh"
 
 #include <cooperative_groups.h>
@@ -635,8 +636,10 @@ int chunk_of(int64_t tokens, int64_t dim) {
 
 // One launch instead of three: up to kFew tokens, half as many above 1024 columns,
 // where the rows of an id that occurs often take longer (one block adds them).
-// A call for 512 rows of 768, ids by word frequency: 10.3 us against 14.8; for 256
-// rows of 4096: 10.3 against 14.8, and of one id for all 256: 37 against 16.
+// Calls for bf16 rows, ids by word frequency, added to a gradient of 32000 or 50257
+// rows: 8 tokens of 768, 7.1 us against 13.9; 512 of 768, 12.6 against 16 to 21; 256 of
+// 4096, 10.4 against 16.2, and of one id for all 256, 43 against 17.  A dense gradient of
+// 50257 rows, which is mostly zeros: 27 against 31, 35.2 against 33.5, 134 against 127.
 bool few(int64_t tokens, int64_t dim) { return tokens <= (dim <= 1024 ? kFew : kFew / 2); }
 
 struct Layout {   // of the workspace

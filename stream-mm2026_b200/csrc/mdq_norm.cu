@@ -321,8 +321,9 @@ struct RowsPlan {
 // 32768 bf16 rows of 2048 / 768 / 128 columns: 96 / 46 / 16 us with two chunks, 126 /
 // 81 / 13 with one, 112 / 50 / 32 with four.
 // Four chunks have their parameters loaded for every row, value by value off 16
-// bytes: rather twice the CTAs then (4112 bf16 rows of 16301: 244 against 553 us),
-// but for fp32 rows without means and biases (6704 of 10001: 355 against 287).
+// bytes: rather twice the CTAs then (4112 bf16 rows of 16301: 235 against 425 us, layer
+// norm 361 against 584), but for fp32 rows without means and biases (6704 of 10001: 343
+// against 318; with them 532 against 498).
 bool plan_forward(int64_t rows, int64_t dim, int64_t row_bytes, bool vec, bool full, RowsPlan* p) {
     const bool ring = full || !vec;
     for (int most = vec || (row_bytes == 8 && !full) ? 4 : 2; most >= 1; most /= 2) {
@@ -385,9 +386,12 @@ bool plan_grad(int64_t rows, int64_t dim, int64_t gate_rows, bool full, GradPlan
     return true;
 }
 // With rows in a ring.  Above 8192 columns the steps between more than two CTAs
-// take longer than the other kernel's rows (440 against 312 us for 4096 bf16 rows of
-// 16384), but not than its loads of rows off 16 bytes (513 against 2549 us for 4112
-// rows of 16301).
+// take longer than the other kernel's rows (431 against 270 us for 4096 bf16 rows of
+// 16384), but not than its loads of rows off 16 bytes (497 against 1597 us for 4112
+// rows of 16301).  Rows off 16 bytes of more than 32768 columns, which no cluster's
+// ring takes, are left to it: calls for 16 / 512 bf16 rows of 33001, 62 / 1163 us, and
+// 512 of 65535, 1319, against 561 / 2053 and 2956 by the kernels for rows wider than a
+// cluster.
 bool plan_stream(int64_t rows, int64_t dim, int64_t gate_rows, int64_t row_bytes, bool vec, bool full,
                  GradPlan* p) {
     p->chunks = 1;

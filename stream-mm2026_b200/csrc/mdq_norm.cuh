@@ -11,9 +11,9 @@
 // the chip and leaves one partial sum for each CTA, which a second kernel adds in a
 // fixed order.
 //
-// Measured, 16384 rows of 4096: bf16 RMS norm forward 96 us (5.6 TB/s), backward 159
-// (5.1 TB/s); layer norm of an fp32 stream and bf16 blocks 168 (4.8) and 222 (5.4).
-// With bf16 alone the steps of a row take longer than its bytes: 153 and 199 us.
+// Measured, 16384 rows of 4096: bf16 RMS norm forward 97 us (5.5 TB/s), backward 150
+// (5.4 TB/s); layer norm of an fp32 stream and bf16 blocks 172 (4.7) and 203 (6.0).
+// With bf16 alone the steps of a row take longer than its bytes: 132 and 185 us.
 #pragma once
 
 #include "mdq_ops.cuh"
@@ -601,8 +601,8 @@ __global__ void __launch_bounds__(kTeam, 1) norm_rows(const __grid_constant__ md
 
 // Layer norm, biases, or rows of any alignment: a team's rows come through a ring
 // of `stages` in shared memory, so that no registers hold loads.  FULL: layer norm
-// or biases.  4096 bf16 rows of 8192, layer norm: 87 us (93 against 115 with rows in
-// registers when both were built); 16368 rows of 1601: 66 (93 against 190).
+// or biases.  4096 bf16 rows of 8192, layer norm: 71 us (93 against 115 with rows in
+// registers when both were built); 16368 rows of 1601: 61 (93 against 190).
 template <typename XT, typename HT, bool VECTOR, int I, bool FULL>
 __global__ void __launch_bounds__(kTeam, 1) norm_rows_ring(const __grid_constant__
                                                            mdq_residual_norm_desc d,

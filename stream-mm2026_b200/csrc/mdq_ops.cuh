@@ -62,8 +62,8 @@ __device__ __forceinline__ void bar_arrive(void* bar) {
 
 // Whether the barrier's phase ended.  Phases last microseconds; the limit
 // (hundreds of milliseconds) only keeps a lost copy from hanging the GPU.  Behind
-// a wait that ran out, nothing that it was for is read, its barrier is not
-// arrived at again, and the results become NaN.
+// a wait that ran out nothing that it was for is used, nothing more is copied, and
+// the results become NaN.
 [[nodiscard]] __device__ __forceinline__ bool bar_wait(void* bar, unsigned parity) {
     for (int i = 0; i < 1 << 22; ++i) {
         unsigned done;

@@ -199,7 +199,9 @@ def scaled_embedding_grad(ids: torch.Tensor, grad_out: torch.Tensor, vocab: int,
     nothing.
 
     ``out`` (contiguous, [vocab, dim]) receives the result; with ``accumulate``
-    (fp32) the sums are added to it, and only the rows that occur are touched.
+    (fp32) the sums are added to it, and only the rows that occur are touched (by
+    additions that take subnormal values as zero).  To autograd that is an in-place
+    operation on ``out``.
     """
     dev = _device(grad_out, "grad_out")
     _no_tangents(grad_out, out)
@@ -561,9 +563,10 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     without an entry above -infinity, has loss and gradient 0, whatever its logits
     hold.  top = 1 with temperature 1 is the cross-entropy against the index.
 
-    ``out`` receives the gradient (logits' shape and dtype, evenly strided rows);
-    it may be ``logits``, which are then overwritten, but share nothing else with them.  Without ``grad`` only the
-    loss is computed."""
+    ``out`` receives the gradient (logits' shape and dtype, evenly strided rows), to
+    autograd an in-place operation on it; it may be ``logits``, which are then
+    overwritten, but share nothing else with them.  Without ``grad`` only the loss is
+    computed."""
     given = out is not None
     if given:
         if not grad:
